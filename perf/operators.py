@@ -7,7 +7,7 @@ Operators (all of `cache_dit_amd.ops`), and what they compute:
       2^(e - 127), e one byte, and each value is one of 0, .5, 1, 1.5, 2, 3, 4, 6 and a sign. Two
       values a byte (the lower half byte is the earlier one). e is the exponent of the block's
       largest magnitude less 2, one more where that magnitude is 1.75 times a power of two or
-      above (it would be cut to 6/7 otherwise), at least 1; values are rounded to the nearest,
+      above (it would be cut to 6/7 otherwise), in 1 .. 252; values are rounded to the nearest,
       ties to the even code. A row of scales has 4 ceil(K / 128) bytes, those behind K / 32 are 127.
   mxfp4_linear
       x W^T + bias (optionally GELU-tanh of it), x quantised per call, W kept in MXFP4.
@@ -148,7 +148,7 @@ def prepare(case, seed):
 def _block_exponents(blocks):
   """The scale bytes of fp32 blocks [..., 32], as int32 [..., 1]; 255 where a value is not finite."""
   top = blocks.abs().amax(-1, keepdim=True)
-  e = (((top.view(torch.int32) + 0x200000) >> 23) - 2).clamp(min=1)
+  e = (((top.view(torch.int32) + 0x200000) >> 23) - 2).clamp(1, 252)
   return torch.where(torch.isfinite(top), e, 255)
 
 
@@ -266,7 +266,7 @@ def _exact_quantised(x):
   b = x.reshape(*x.shape[:-1], -1, 32)
   mantissa, exponent = torch.frexp(b.abs().amax(-1, keepdim=True))  # mantissa in [.5, 1)
   exponent = torch.where(mantissa >= 0.875, exponent + 1, exponent) - 1 - 2
-  scale = torch.exp2(exponent.clamp(min=-126).double())
+  scale = torch.exp2(exponent.clamp(-126, 125).double())
   grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64, device=x.device)
   a = b.abs() / scale
   above = torch.searchsorted(grid, a).clamp(1, 7)  # grid[above - 1] < a <= grid[above]
