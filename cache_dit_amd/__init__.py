@@ -6,7 +6,8 @@ cache-dit's `quantize()` / `enable_cache(..., quantize_config=...)` API.
 
 Built quant types: `float8_per_row` (w8a8, dynamic per-token activation scales),
 `float8_per_tensor` (w8a8, one dynamic scale per tensor; also the policy's fallback
-pass) and `float8_weight_only` (w8a16). The kernels live in lib/libcdit_hip.so
+pass), `float8_weight_only` (w8a16), `mxfp4` (w4a4: weights and activations in microscaled 4-bit
+floating point) and `mxfp4_weight_only` (w4a16). The kernels live in lib/libcdit_hip.so
 (C ABI: include/cdit_hip.h); there is no CPU or eager fallback.
 """
 from .quantization import QuantizeBackend
@@ -19,6 +20,8 @@ from .caching import load_quantize_config
 from .nn import Fp8DynamicLinear
 from .nn import Fp8DynamicLinearPerTensor
 from .nn import Fp8WeightOnlyLinear
+from .nn import Mxfp4Linear
+from .nn import Mxfp4WeightOnlyLinear
 from .nn import fuse_gelu_tanh_
 from .nn import share_activation_quant_
 from .nn import group_sibling_linears_
@@ -29,6 +32,10 @@ from .patch_functors import StagePatchFunctor
 from .patch_functors import apply_stage_patch
 from .patch_functors import remove_stage_patch
 from .ops import ln_modulate_quant
+from .mxfp4 import gate_residual_norm
+from .mxfp4 import mxfp4_quant
+from .mxfp4 import mxfp4_dequant
+from .mxfp4 import mxfp4_mm
 from .utils import check_quantized
 
 __version__ = "0.1.0"
@@ -55,4 +62,10 @@ __all__ = [
     "apply_stage_patch",
     "remove_stage_patch",
     "ln_modulate_quant",
+    "Mxfp4Linear",
+    "Mxfp4WeightOnlyLinear",
+    "gate_residual_norm",
+    "mxfp4_quant",
+    "mxfp4_dequant",
+    "mxfp4_mm",
 ]

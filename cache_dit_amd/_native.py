@@ -49,6 +49,12 @@ EXPORTS = (
     "cdit_fp8_comm_per_token_dequant",
     "cdit_fp8_comm_qkv_permute_quant",
     "cdit_fp8_comm_qkv_permute_dequant",
+    "cdit_mxfp4_quant",
+    "cdit_mxfp4_dequant",
+    "cdit_mxfp4_gemm",
+    "cdit_mxfp4_linear",
+    "cdit_w4a16_gemm",
+    "cdit_gate_residual_norm",
     "cdit_debug_set_gemm_variant",
     "cdit_debug_set_quant_hints",
     "cdit_debug_gemm_choice",
@@ -130,6 +136,18 @@ def _bind(L: ctypes.CDLL) -> None:
   L.cdit_fp8_comm_qkv_permute_quant.argtypes = [vp, i64, i64, i64, i64, i64, i64, i64, i64, vp, vp]
   L.cdit_fp8_comm_qkv_permute_dequant.restype = ci
   L.cdit_fp8_comm_qkv_permute_dequant.argtypes = [vp, i64, i64, i64, i64, i64, i64, i64, vp, vp]
+  L.cdit_mxfp4_quant.restype = ci
+  L.cdit_mxfp4_quant.argtypes = [vp, ci, i64, i64, i64, vp, i64, vp, i64, vp]
+  L.cdit_mxfp4_dequant.restype = ci
+  L.cdit_mxfp4_dequant.argtypes = [vp, i64, vp, i64, i64, i64, vp, ci, i64, vp]
+  L.cdit_mxfp4_gemm.restype = ci
+  L.cdit_mxfp4_gemm.argtypes = [vp] * 6 + [i64] * 8 + [ci, ci, vp]
+  L.cdit_mxfp4_linear.restype = ci
+  L.cdit_mxfp4_linear.argtypes = [vp] * 7 + [i64] * 7 + [ci, vp]
+  L.cdit_w4a16_gemm.restype = ci
+  L.cdit_w4a16_gemm.argtypes = [vp] * 5 + [i64] * 7 + [ci, vp]
+  L.cdit_gate_residual_norm.restype = ci
+  L.cdit_gate_residual_norm.argtypes = [vp, vp]
   L.cdit_w8a16_gemm_batched.restype = ci
   L.cdit_w8a16_gemm_batched.argtypes = [ci, vp, vp, i64, i64, vp, vp, vp, vp, vp, vp, i64, vp, vp, vp]
   L.cdit_w8a16_gemm.restype = ci

@@ -1,0 +1,261 @@
+// What stands between two branches of a transformer block (include/cdit_hip.h, cdit_gate_residual_norm): the
+// branch's own norm, its gate, the residual sum, the next norm and its modulation in one pass, and the MXFP4 codes
+// of the result where a 4-bit Linear reads it. Bound by HBM: x and the branch are read once, h and y written once.
+//
+//   t = branch                      or  w_post * branch / sqrt(mean(branch^2) + eps)   (or LayerNorm of it)
+//   h = r x + gate t
+//   y = norm(h) [* w] [* (1 + scale)] [+ shift]
+//
+// All in fp32 from the loads to the two roundings at the end: h is rounded to the stream's type where it is stored,
+// and y is computed from the unrounded h, so that a 16-bit stream costs the norm nothing.
+#include "gemm_common.h"
+#include "mxfp4_device.h"
+#include "quant_device.h"
+
+namespace cdit {
+namespace {
+
+typedef cdit_gate_residual_norm_args Args;
+
+template <int DT>
+__device__ __forceinline__ void widen8(const Mx8<DT>& v, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (DT == CDIT_DT_F32) {
+      f[i] = __uint_as_float(v.w[i]);
+    } else if constexpr (DT == CDIT_DT_BF16) {
+      f[i] = i & 1 ? bf16_hi(v.w[i / 2]) : bf16_lo(v.w[i / 2]);
+    } else {
+      f[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(v.w[i / 2] >> (16 * (i & 1))));
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ Mx8<DT> narrow8(const float (&f)[8]) {
+  Mx8<DT> v;
+  if constexpr (DT == CDIT_DT_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.w[i] = __float_as_uint(f[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v.w[i] = DT == CDIT_DT_BF16 ? pack_bf16x2(f[2 * i], f[2 * i + 1]) : pack_f16x2(f[2 * i], f[2 * i + 1]);
+  }
+  return v;
+}
+template <int DT>
+__host__ __device__ constexpr int size_of() {
+  return DT == CDIT_DT_F32 ? 4 : 2;
+}
+
+// n <= 8 elements at p, the others zero. VEC: n is 0 or 8 and p is 16-byte aligned.
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const void* p, int n, float (&f)[8]) {
+  if constexpr (VEC) {
+    Mx8<DT> v = {};
+    if (n > 0) v = mx_load8<DT>(p);
+    widen8<DT>(v, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[i] = 0.0f;
+      if (i >= n) continue;
+      if constexpr (DT == CDIT_DT_F32) {
+        f[i] = static_cast<const float*>(p)[i];
+      } else if constexpr (DT == CDIT_DT_BF16) {
+        f[i] = __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
+      } else {
+        f[i] = (float)static_cast<const _Float16*>(p)[i];
+      }
+    }
+  }
+}
+template <int DT, bool VEC>
+__device__ __forceinline__ void store8(void* p, int n, const float (&f)[8]) {
+  const Mx8<DT> v = narrow8<DT>(f);
+  if constexpr (VEC) {
+    if (n > 0) mx_store8<DT>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i >= n) continue;
+      if constexpr (DT == CDIT_DT_F32) {
+        static_cast<uint32_t*>(p)[i] = v.w[i];
+      } else {
+        static_cast<uint16_t*>(p)[i] = (uint16_t)(v.w[i / 2] >> (16 * (i & 1)));
+      }
+    }
+  }
+}
+
+// Sums over a workgroup of WAVES wavefronts, in an order of their own that does not change from call to call.
+template <int WAVES>
+struct BlockSum {
+  float (*slot)[WAVES];  // two sets in turn: a set is read by all before the one after next is written
+  int turn;
+  __device__ __forceinline__ float operator()(float v) {
+    v = wave_sum_f32(v);
+    if constexpr (WAVES > 1) {
+      float* const s = slot[turn];
+      turn ^= 1;
+      if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+      __syncthreads();
+      v = s[0];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) v += s[w];
+    }
+    return v;
+  }
+};
+
+// A piece of 8 columns of the row: where it is, and what of it exists.
+template <int ST, int DT, bool VEC>
+struct Row {
+  const Args& a;
+  int64_t row;
+  __device__ __forceinline__ int n_of(int c) const { return min(max((int)a.K - 8 * c, 0), 8); }
+  __device__ __forceinline__ void vec(const void* p, int64_t ld, int64_t rows_per, int c, float (&f)[8]) const {
+    const int64_t at = (rows_per > 0 ? row / rows_per * ld : 0) + 8 * c;
+    if (a.vec_f32)
+      load8<CDIT_DT_F32, VEC>(static_cast<const float*>(p) + at, n_of(c), f);
+    else
+      load8<DT, VEC>(static_cast<const uint8_t*>(p) + at * size_of<DT>(), n_of(c), f);
+  }
+  __device__ __forceinline__ void branch(int c, float (&t)[8]) const {
+    load8<DT, VEC>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + 8 * c) * size_of<DT>(), n_of(c), t);
+  }
+  // t -> post norm of t; mean and rstd of the branch's row
+  __device__ __forceinline__ void post(int c, float mean, float rstd, float (&t)[8]) const {
+    float w[8];
+    if (a.post_weight) vec(a.post_weight, 0, 0, c, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = (t[i] - mean) * rstd * (a.post_weight ? w[i] : 1.0f);
+  }
+  // t -> h
+  __device__ __forceinline__ void residual(int c, float (&t)[8]) const {
+    float x[8], g[8];
+    load8<ST, VEC>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + 8 * c) * size_of<ST>(), n_of(c), x);
+    if (a.gate) vec(a.gate, a.ld_gate, a.rows_per_gate, c, g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = __fmaf_rn(a.gate ? g[i] : 1.0f, t[i], a.residual_scale * x[i]);
+  }
+  // h -> h stored; h -> y stored, or its codes
+  __device__ __forceinline__ void finish(int c, float mean, float rstd, const float (&h)[8]) const {
+    const int n = n_of(c);
+    float y[8], f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = (h[i] - mean) * rstd;
+    if (a.norm_weight) {
+      vec(a.norm_weight, 0, 0, c, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] *= f[i];
+    }
+    if (a.scale) {
+      vec(a.scale, a.ld_scale, a.rows_per_scale, c, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __fmaf_rn(y[i], f[i], y[i]);
+    }
+    if (a.shift) {
+      vec(a.shift, a.ld_shift, a.rows_per_shift, c, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] += f[i];
+    }
+    store8<ST, VEC>(static_cast<uint8_t*>(a.h) + (row * a.ld_h + 8 * c) * size_of<ST>(), n, h);
+    if (a.y) store8<DT, VEC>(static_cast<uint8_t*>(a.y) + (row * a.ld_y + 8 * c) * size_of<DT>(), n, y);
+    if (a.codes) {
+      // the codes of y as it is (or would be) stored; K is a multiple of 32, so that the quad of lanes
+      // that holds a block is in the row as a whole
+      const Mx8<DT> v = narrow8<DT>(y);
+      const int e = mx_exponent(mx_quad_max(mx_amax8<DT>(v)));
+      if (n > 0) {
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.codes) + row * a.ld_codes + 4 * c) = mx_codes8<DT>(v, e);
+        uint8_t* const s = static_cast<uint8_t*>(a.code_scales) + row * a.ld_code_scales;
+        if (c % 4 == 0) {
+          const int b = c / 4, blocks = (int)a.K / kMxBlock;
+          s[b] = (uint8_t)e;
+          if (b == blocks - 1)
+            for (int pad = blocks; pad % 4 != 0; ++pad) s[pad] = (uint8_t)kMxPad;
+        }
+      }
+    }
+  }
+};
+
+// Mean (0 for RMS) and 1 / sqrt(variance or mean square + eps) of a row; `piece(c, f)` gives its pieces. The squares
+// are those of the values less the mean: no cancellation, whatever the row's offset.
+template <class Piece, class Sum>
+__device__ __forceinline__ void statistics(const Args& a, bool layer, Sum& sum, int first, int step, int pieces, Piece piece,
+                                           float* mean, float* rstd) {
+  const float inv_k = 1.0f / (float)a.K;
+  float s = 0.0f;
+  *mean = 0.0f;
+  if (layer) {
+    for (int c = first; c < pieces; c += step) {
+      float f[8];
+      piece(c, f);
+      const int n = min((int)a.K - 8 * c, 8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += i < n ? f[i] : 0.0f;
+    }
+    *mean = sum(s) * inv_k;
+    s = 0.0f;
+  }
+  for (int c = first; c < pieces; c += step) {
+    float f[8];
+    piece(c, f);
+    const int n = min((int)a.K - 8 * c, 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float d = i < n ? f[i] - *mean : 0.0f;
+      s = __fmaf_rn(d, d, s);
+    }
+  }
+  *rstd = 1.0f / __fsqrt_rn(sum(s) * inv_k + a.eps);
+}
+
+// A workgroup per row, the row read again in each pass: any K, any stride and alignment.
+template <int ST, int DT>
+__global__ __launch_bounds__(256) void gate_residual_norm_any(Args a) {
+  __shared__ float slots[2][4];
+  BlockSum<4> sum{slots, 0};
+  const int pieces = (int)((a.K + 7) / 8);
+  // (whole quads of lanes take part in a block's maximum, also behind the last piece)
+  for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+    const Row<ST, DT, false> r{a, row};
+    float pm = 0.0f, pr = 1.0f, mean, rstd;
+    if (a.post_norm)
+      statistics(a, a.post_norm == CDIT_NORM_LAYER, sum, threadIdx.x, 256, pieces,
+                 [&](int c, float(&f)[8]) { r.branch(c, f); }, &pm, &pr);
+    auto h_of = [&](int c, float(&f)[8]) {
+      r.branch(c, f);
+      if (a.post_norm) r.post(c, pm, pr, f);
+      r.residual(c, f);
+    };
+    statistics(a, a.norm == CDIT_NORM_LAYER, sum, threadIdx.x, 256, pieces, h_of, &mean, &rstd);
+    for (int c = threadIdx.x; c < pieces; c += 256) {
+      float h[8];
+      h_of(c, h);
+      r.finish(c, mean, rstd, h);
+    }
+  }
+}
+
+template <int ST, int DT>
+int launch_types(const Args& a, hipStream_t stream) {
+  const dim3 grid((unsigned)std::min<int64_t>(a.M, 1 << 20));
+  hipLaunchKernelGGL((gate_residual_norm_any<ST, DT>), grid, dim3(256), 0, stream, a);
+  return 0;
+}
+
+}  // namespace
+
+int launch_gate_residual_norm(const Args& a, hipStream_t stream) {
+  if (a.dtype == CDIT_DT_F32) return launch_types<CDIT_DT_F32, CDIT_DT_F32>(a, stream);
+  if (a.dtype == CDIT_DT_BF16)
+    return a.x_dtype == CDIT_DT_F32 ? launch_types<CDIT_DT_F32, CDIT_DT_BF16>(a, stream)
+                                    : launch_types<CDIT_DT_BF16, CDIT_DT_BF16>(a, stream);
+  return a.x_dtype == CDIT_DT_F32 ? launch_types<CDIT_DT_F32, CDIT_DT_F16>(a, stream)
+                                  : launch_types<CDIT_DT_F16, CDIT_DT_F16>(a, stream);
+}
+
+}  // namespace cdit

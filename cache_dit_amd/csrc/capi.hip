@@ -634,6 +634,207 @@ int cdit_fp8_linear_w8a8(const void* x_bf16, const void* w_q, const float* w_sca
                                epilogue, out_dtype_id, stream);
 }
 
+// ---- MXFP4
+static bool known_dtype(int id) { return id == CDIT_DT_F16 || id == CDIT_DT_BF16 || id == CDIT_DT_F32; }
+static int64_t mx_scale_bytes(int64_t K) { return (K + 127) / 128 * 4; }
+static bool on(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// A matrix in MXFP4: codes on `align` bytes.
+static int check_mx(const char* fn, const char* what, const void* codes, const void* scales, int64_t rows, int64_t K,
+                    int64_t ld_codes, int64_t ld_scales, int align) {
+  if (rows < 0 || K < 0 || rows > INT32_MAX || K > INT32_MAX - 512) {
+    set_error("%s: bad shape of %s (%lld x %lld)", fn, what, (long long)rows, (long long)K);
+    return CDIT_EINVAL;
+  }
+  if (K % 32 != 0) {
+    set_error("%s: K=%lld is not a multiple of 32", fn, (long long)K);
+    return CDIT_EINVAL;
+  }
+  if (ld_codes < K / 2 || ld_scales < mx_scale_bytes(K)) {
+    set_error("%s: leading dimension of %s smaller than the row (codes %lld, scales %lld)", fn, what, (long long)ld_codes,
+              (long long)ld_scales);
+    return CDIT_EINVAL;
+  }
+  if (ld_codes % align != 0 || ld_scales % 4 != 0 || !on(codes, align) || !on(scales, 4)) {
+    set_error("%s: rows of %s must start on %d bytes (codes) and 4 bytes (scales)", fn, what, align);
+    return CDIT_EINVAL;
+  }
+  if (rows > 0 && K > 0 && (!codes || !scales)) {
+    set_error("%s: null pointer argument", fn);
+    return CDIT_EINVAL;
+  }
+  return CDIT_OK;
+}
+static int check_mx_dense(const char* fn, const void* p, int64_t rows, int64_t K, int64_t ld, int dtype_id) {
+  if (!known_dtype(dtype_id)) {
+    set_error("%s: unknown dtype id %d (0 = fp16, 1 = bf16, 2 = fp32)", fn, dtype_id);
+    return CDIT_EINVAL;
+  }
+  if (ld < K) {
+    set_error("%s: leading dimension %lld smaller than the row (%lld)", fn, (long long)ld, (long long)K);
+    return CDIT_EINVAL;
+  }
+  if (!on(p, 16) || ld * (dtype_id == CDIT_DT_F32 ? 4 : 2) % 16 != 0) {
+    set_error("%s: rows must start on 16 bytes", fn);
+    return CDIT_EINVAL;
+  }
+  if (rows > 0 && K > 0 && !p) {
+    set_error("%s: null pointer argument", fn);
+    return CDIT_EINVAL;
+  }
+  return CDIT_OK;
+}
+
+int cdit_mxfp4_quant(const void* x, int x_dtype_id, int64_t M, int64_t K, int64_t ld_x, void* codes, int64_t ld_codes,
+                     void* scales, int64_t ld_scales, void* stream) {
+  const char* fn = "cdit_mxfp4_quant";
+  int rc = check_mx(fn, "the codes", codes, scales, M, K, ld_codes, ld_scales, 4);
+  if (rc || (rc = check_mx_dense(fn, x, M, K, ld_x, x_dtype_id))) return rc;
+  if (M == 0 || K == 0) return CDIT_OK;
+  if ((rc = check_arch())) return rc;
+  rc = launch_mxfp4_quant(x, x_dtype_id, M, K, ld_x, codes, ld_codes, scales, ld_scales,
+                          static_cast<hipStream_t>(stream));
+  return rc ? rc : after_launch(fn);
+}
+
+int cdit_mxfp4_dequant(const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int64_t M, int64_t K,
+                       void* out, int out_dtype_id, int64_t ld_out, void* stream) {
+  const char* fn = "cdit_mxfp4_dequant";
+  int rc = check_mx(fn, "the codes", codes, scales, M, K, ld_codes, ld_scales, 4);
+  if (rc || (rc = check_mx_dense(fn, out, M, K, ld_out, out_dtype_id))) return rc;
+  if (M == 0 || K == 0) return CDIT_OK;
+  if ((rc = check_arch())) return rc;
+  rc = launch_mxfp4_dequant(codes, ld_codes, scales, ld_scales, M, K, out, out_dtype_id, ld_out,
+                            static_cast<hipStream_t>(stream));
+  return rc ? rc : after_launch(fn);
+}
+
+// What both 4-bit GEMMs ask of the weight and the output.
+static int check_mx_gemm(const char* fn, const void* w, const void* ws, const void* out, int64_t M, int64_t N, int64_t K,
+                         int64_t ldw, int64_t ldws, int64_t ldo, int epilogue, int out_dtype_id) {
+  if (M < 0 || M > INT32_MAX - 512 || N > INT32_MAX - 512) {
+    set_error("%s: bad shape (M=%lld N=%lld)", fn, (long long)M, (long long)N);
+    return CDIT_EINVAL;
+  }
+  if (int rc = check_mx(fn, "the weight", w, ws, N, K, ldw, ldws, 16)) return rc;
+  if (!known_dtype(out_dtype_id)) {
+    set_error("%s: unknown out_dtype_id %d (0 = fp16, 1 = bf16, 2 = fp32)", fn, out_dtype_id);
+    return CDIT_EINVAL;
+  }
+  if (epilogue & ~CDIT_EPI_GELU_TANH) {
+    set_error("%s: unknown epilogue bits 0x%x", fn, epilogue);
+    return CDIT_EINVAL;
+  }
+  if (ldo < N) {
+    set_error("%s: ldo=%lld is smaller than the row (%lld)", fn, (long long)ldo, (long long)N);
+    return CDIT_EINVAL;
+  }
+  if (M > 0 && N > 0 && !out) {
+    set_error("%s: null pointer argument", fn);
+    return CDIT_EINVAL;
+  }
+  return CDIT_OK;
+}
+
+int cdit_mxfp4_gemm(const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales, const void* bias,
+                    void* out, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldas, int64_t ldb, int64_t ldbs,
+                    int64_t ldo, int epilogue, int out_dtype_id, void* stream) {
+  const char* fn = "cdit_mxfp4_gemm";
+  int rc = check_mx_gemm(fn, b_codes, b_scales, out, M, N, K, ldb, ldbs, ldo, epilogue, out_dtype_id);
+  if (rc || (rc = check_mx(fn, "the activation", a_codes, a_scales, M, K, lda, ldas, 16))) return rc;
+  if (M == 0 || N == 0) return CDIT_OK;
+  if ((rc = check_arch())) return rc;
+  const Mx4Gemm g{static_cast<const uint8_t*>(a_codes), static_cast<const uint8_t*>(a_scales),
+                  static_cast<const uint8_t*>(b_codes), static_cast<const uint8_t*>(b_scales), bias, out, (int)M, (int)N,
+                  (int)K, lda, ldas, ldb, ldbs, ldo, epilogue, out_dtype_id};
+  rc = launch_gemm_mxfp4(g, static_cast<hipStream_t>(stream));
+  return rc ? rc : after_launch(fn);
+}
+
+int cdit_mxfp4_linear(const void* x_bf16, const void* w_codes, const void* w_scales, const void* bias_bf16, void* out,
+                      void* codes_ws, void* scales_ws, int64_t M, int64_t N, int64_t K, int64_t ld_x, int64_t ldw,
+                      int64_t ldws, int64_t ldo, int epilogue, void* stream) {
+  const char* fn = "cdit_mxfp4_linear";
+  int rc = check_mx_gemm(fn, w_codes, w_scales, out, M, N, K, ldw, ldws, ldo, epilogue, CDIT_DT_BF16);
+  if (rc || (rc = check_mx(fn, "the workspaces", codes_ws, scales_ws, M, K, K / 2, mx_scale_bytes(K), 16))) return rc;
+  if ((rc = cdit_mxfp4_quant(x_bf16, CDIT_DT_BF16, M, K, ld_x, codes_ws, K / 2, scales_ws, mx_scale_bytes(K), stream)))
+    return rc;
+  return cdit_mxfp4_gemm(codes_ws, scales_ws, w_codes, w_scales, bias_bf16, out, M, N, K, K / 2, mx_scale_bytes(K), ldw,
+                         ldws, ldo, epilogue, CDIT_DT_BF16, stream);
+}
+
+int cdit_w4a16_gemm(const void* x_bf16, const void* w_codes, const void* w_scales, const void* bias_bf16, void* out,
+                    int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldw, int64_t ldws, int64_t ldo, int epilogue,
+                    void* stream) {
+  const char* fn = "cdit_w4a16_gemm";
+  int rc = check_mx_gemm(fn, w_codes, w_scales, out, M, N, K, ldw, ldws, ldo, epilogue, CDIT_DT_BF16);
+  if (rc || (rc = check_mx_dense(fn, x_bf16, M, K, lda, CDIT_DT_BF16))) return rc;
+  if (M == 0 || N == 0) return CDIT_OK;
+  if ((rc = check_arch())) return rc;
+  const Mx4Gemm g{static_cast<const uint8_t*>(x_bf16), nullptr, static_cast<const uint8_t*>(w_codes),
+                  static_cast<const uint8_t*>(w_scales), bias_bf16, out, (int)M, (int)N, (int)K, lda, 0, ldw, ldws, ldo,
+                  epilogue, CDIT_DT_BF16};
+  rc = launch_gemm_w4a16(g, static_cast<hipStream_t>(stream));
+  return rc ? rc : after_launch(fn);
+}
+
+// ---- the block norm
+int cdit_gate_residual_norm(const cdit_gate_residual_norm_args* args, void* stream) {
+  const char* fn = "cdit_gate_residual_norm";
+  if (!args) {
+    set_error("%s: null pointer argument", fn);
+    return CDIT_EINVAL;
+  }
+  const cdit_gate_residual_norm_args& a = *args;
+  if (a.M < 0 || a.K < 0 || a.K > INT32_MAX - 16384) {
+    set_error("%s: bad shape M=%lld K=%lld", fn, (long long)a.M, (long long)a.K);
+    return CDIT_EINVAL;
+  }
+  if (!known_dtype(a.dtype) || (a.x_dtype != a.dtype && a.x_dtype != CDIT_DT_F32)) {
+    set_error("%s: x_dtype %d with dtype %d (0 = fp16, 1 = bf16, 2 = fp32; x has the branch's or fp32)", fn, a.x_dtype,
+              a.dtype);
+    return CDIT_EINVAL;
+  }
+  if ((a.norm != CDIT_NORM_LAYER && a.norm != CDIT_NORM_RMS) ||
+      (a.post_norm != CDIT_NORM_NONE && a.post_norm != CDIT_NORM_LAYER && a.post_norm != CDIT_NORM_RMS)) {
+    set_error("%s: unknown norm %d / post_norm %d", fn, a.norm, a.post_norm);
+    return CDIT_EINVAL;
+  }
+  if (a.post_weight && a.post_norm == CDIT_NORM_NONE) {
+    set_error("%s: post_weight without post_norm", fn);
+    return CDIT_EINVAL;
+  }
+  if (!(a.eps >= 0.0f)) {
+    set_error("%s: eps must not be negative", fn);
+    return CDIT_EINVAL;
+  }
+  if (a.M == 0 || a.K == 0) return CDIT_OK;
+  if (a.ld_x < a.K || a.ld_branch < a.K || a.ld_h < a.K || (a.y && a.ld_y < a.K)) {
+    set_error("%s: leading dimension smaller than the row", fn);
+    return CDIT_EINVAL;
+  }
+  if ((a.gate && a.rows_per_gate < 1) || (a.shift && a.rows_per_shift < 1) || (a.scale && a.rows_per_scale < 1)) {
+    set_error("%s: rows_per_* must be at least 1", fn);
+    return CDIT_EINVAL;
+  }
+  if (!a.x || !a.branch || !a.h || (!a.y && !a.codes)) {
+    set_error("%s: null pointer argument", fn);
+    return CDIT_EINVAL;
+  }
+  const int es = a.dtype == CDIT_DT_F32 ? 4 : 2, vs = a.vec_f32 ? 4 : es, ss = a.x_dtype == CDIT_DT_F32 ? 4 : 2;
+  if (!on(a.x, ss) || !on(a.h, ss) || !on(a.branch, es) || !on(a.y, es) || !on(a.gate, vs) || !on(a.shift, vs) ||
+      !on(a.scale, vs) || !on(a.norm_weight, vs) || !on(a.post_weight, vs)) {
+    set_error("%s: misaligned pointer", fn);
+    return CDIT_EINVAL;
+  }
+  int rc = CDIT_OK;
+  if (a.codes && (rc = check_mx(fn, "the codes", a.codes, a.code_scales, a.M, a.K, a.ld_codes, a.ld_code_scales, 4)))
+    return rc;
+  if ((rc = check_arch())) return rc;
+  rc = launch_gate_residual_norm(a, static_cast<hipStream_t>(stream));
+  return rc ? rc : after_launch(fn);
+}
+
 // ---- FP8 quantizers with packed trailing scales (activations that cross GPUs)
 static int check_comm(const char* fn, const void* in, const void* out, int64_t rows, int64_t width,
                       int64_t min_width) {

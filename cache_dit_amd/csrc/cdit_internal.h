@@ -121,6 +121,29 @@ int launch_gemm_w8a16_grouped(const GemmArgs& common, const GemmGroup& grp, int 
 int launch_linear_fp8_skinny_fused(const GemmArgs& g, void* q_ws, float* scale_ws, int scale_mode,
                                    int variant, hipStream_t stream);
 
+// MXFP4 (mxfp4_quant.hip, gemm_mxfp4.hip, gemm_w4a16.hip). dtype: CDIT_DT_* of the side that is not in
+// 4 bits; leading dimensions of codes and scales in bytes.
+int launch_mxfp4_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ld_x, void* codes, int64_t ld_codes,
+                       void* scales, int64_t ld_scales, hipStream_t stream);
+int launch_mxfp4_dequant(const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int64_t M, int64_t K,
+                         void* out, int dtype, int64_t ld_out, hipStream_t stream);
+struct Mx4Gemm {
+  const uint8_t* a;        // codes [M, K/2] (w4a4) or bf16 [M, K] (w4a16)
+  const uint8_t* a_scale;  // scales of the codes, or nullptr
+  const uint8_t* b;        // codes [N, K/2]
+  const uint8_t* b_scale;
+  const void* bias;        // [N] of the output's dtype, or nullptr
+  void* out;               // [M, N] of out_dtype
+  int M, N, K;
+  int64_t lda, ldas, ldb, ldbs, ldo;  // a: bytes (w4a4) or elements (w4a16); ldo: elements; the others bytes
+  int epilogue, out_dtype;
+};
+int launch_gemm_mxfp4(const Mx4Gemm& g, hipStream_t stream);
+int launch_gemm_w4a16(const Mx4Gemm& g, hipStream_t stream);
+
+// What stands between two branches of a block (block_norm.hip); the arguments are checked by the caller.
+int launch_gate_residual_norm(const cdit_gate_residual_norm_args& a, hipStream_t stream);
+
 // FP8 quantizers with the scale packed behind each row (comm_quant.hip).
 int launch_comm_per_token_quant(const void* x, int64_t M, int64_t H, void* y, hipStream_t stream);
 int launch_comm_per_token_dequant(const void* x, int64_t M, int64_t H, void* y, hipStream_t stream);

@@ -50,6 +50,12 @@ struct Library {
   decltype(&cdit_fp8_comm_per_token_dequant) comm_per_token_dequant;
   decltype(&cdit_fp8_comm_qkv_permute_quant) comm_qkv_permute_quant;
   decltype(&cdit_fp8_comm_qkv_permute_dequant) comm_qkv_permute_dequant;
+  decltype(&cdit_mxfp4_quant) mxfp4_quant;
+  decltype(&cdit_mxfp4_dequant) mxfp4_dequant;
+  decltype(&cdit_mxfp4_gemm) mxfp4_gemm;
+  decltype(&cdit_mxfp4_linear) mxfp4_linear;
+  decltype(&cdit_w4a16_gemm) w4a16_gemm;
+  decltype(&cdit_gate_residual_norm) gate_residual_norm;
 };
 Library lib = {};
 
@@ -593,6 +599,223 @@ PyObject* comm_qkv_permute_dequant(PyObject*, PyObject* const* a, Py_ssize_t n) 
   END_HANDLE_TH_ERRORS
 }
 
+// ---- MXFP4: codes [..., K/2], scales [..., 4 ceil(K/128)], both bytes
+int64_t mx_scale_bytes(int64_t K) { return (K + 127) / 128 * 4; }
+int dtype_id(at::ScalarType t) { return t == at::kHalf ? CDIT_DT_F16 : t == kBf16 ? CDIT_DT_BF16 : t == kF32 ? CDIT_DT_F32 : -1; }
+at::ScalarType dtype_of(int64_t id) { return id == CDIT_DT_F16 ? at::kHalf : id == CDIT_DT_BF16 ? kBf16 : kF32; }
+
+// The rows of any tensor whose leading dimensions, those of one element aside, walk memory in equal steps: a matrix, a
+// contiguous tensor, a slice [:, n:] of one batch entry.
+bool even_rows(const at::Tensor& t, Rows* r) {
+  const int64_t d = t.dim();
+  if (d < 1 || t.size(d - 1) <= 0 || t.stride(d - 1) != 1) return false;
+  r->K = t.size(d - 1);
+  r->M = 1;
+  r->ld = r->K;
+  for (int64_t i = d - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (r->M == 1)
+      r->ld = t.stride(i);
+    else if (t.stride(i) != r->ld * r->M)
+      return false;
+    r->M *= t.size(i);
+  }
+  return true;
+}
+
+// Rows of fp16, bf16 or fp32 that start on 16 bytes.
+bool dense_rows(const at::Tensor& t, Rows* r) {
+  return dtype_id(t.scalar_type()) >= 0 && even_rows(t, r) && r->M > 0 && r->ld >= r->K &&
+         r->ld * (int64_t)t.element_size() % 16 == 0 && aligned16(t);
+}
+// A matrix in MXFP4 on `align` bytes: its rows, K (the elements), and the leading dimensions.
+struct MxRows {
+  int64_t M, K, ld, lds;
+};
+bool mx_rows(const at::Tensor& codes, const at::Tensor& scales, int align, MxRows* m) {
+  Rows c, s;
+  if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kByte || !even_rows(codes, &c) || !even_rows(scales, &s) ||
+      c.M <= 0 || s.M != c.M || c.K % 16 || s.K != mx_scale_bytes(2 * c.K) || c.ld < c.K || s.ld < s.K || c.ld % align ||
+      s.ld % 4 || reinterpret_cast<uintptr_t>(codes.data_ptr()) % align ||
+      reinterpret_cast<uintptr_t>(scales.data_ptr()) % 4 || scales.device() != codes.device())
+    return false;
+  *m = {c.M, 2 * c.K, c.ld, s.ld};
+  return true;
+}
+bool mx_bias(PyObject* o, at::ScalarType type, int64_t N, const at::Tensor& x, void** bias) {
+  *bias = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor& t = tensor(o);
+  if (!vector_of(t, type, N) || t.device() != x.device() || !aligned16(t)) return false;
+  *bias = t.data_ptr();
+  return true;
+}
+
+// mxfp4_quant(x) -> (status, codes, scales)
+PyObject* mxfp4_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 1);
+  const at::Tensor& x = tensor(a[0]);
+  Rows r;
+  if (!dense_rows(x, &r) || r.K % 32) Py_RETURN_NONE;
+  const at::Tensor q = empty_like_rows(x, r.K / 2, at::kByte), s = empty_like_rows(x, mx_scale_bytes(r.K), at::kByte);
+  return with_status(status_of(x, lib.mxfp4_quant, x.data_ptr(), dtype_id(x.scalar_type()), r.M, r.K, r.ld, q.data_ptr(),
+                               r.K / 2, s.data_ptr(), mx_scale_bytes(r.K)), {q, s});
+  END_HANDLE_TH_ERRORS
+}
+// mxfp4_dequant(codes, scales, dtype_id) -> (status, out)
+PyObject* mxfp4_dequant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 3);
+  const at::Tensor &q = tensor(a[0]), &s = tensor(a[1]);
+  const int64_t id = integer(a[2]);
+  MxRows m;
+  if (id < 0 || id > 2 || !mx_rows(q, s, 4, &m)) Py_RETURN_NONE;
+  const at::Tensor out = empty_like_rows(q, m.K, dtype_of(id));
+  return with_status(status_of(q, lib.mxfp4_dequant, q.data_ptr(), m.ld, s.data_ptr(), m.lds, m.M, m.K, out.data_ptr(),
+                               (int)id, m.K), {out});
+  END_HANDLE_TH_ERRORS
+}
+// mxfp4_mm(a_codes, a_scales, b_codes, b_scales, bias, out_dtype_id, epilogue) -> (status, out)
+PyObject* mxfp4_mm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 7);
+  const at::Tensor &x = tensor(a[0]), &xs = tensor(a[1]), &w = tensor(a[2]), &ws = tensor(a[3]);
+  const int64_t id = integer(a[5]);
+  const int epi = (int)integer(a[6]);
+  MxRows m, v;
+  void* bias;
+  if (id < 0 || id > 2 || w.dim() != 2 || !mx_rows(x, xs, 16, &m) || !mx_rows(w, ws, 16, &v) || m.K != v.K ||
+      x.device() != w.device() || !mx_bias(a[4], dtype_of(id), v.M, x, &bias))
+    Py_RETURN_NONE;
+  const at::Tensor out = empty_like_rows(x, v.M, dtype_of(id));
+  return with_status(status_of(x, lib.mxfp4_gemm, x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), bias,
+                               out.data_ptr(), m.M, v.M, m.K, m.ld, m.lds, v.ld, v.lds, v.M, epi, (int)id), {out});
+  END_HANDLE_TH_ERRORS
+}
+// mxfp4_linear(x, weight, weight_scale, bias, epilogue) -> (status, out); the workspaces are one allocation
+PyObject* mxfp4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 5);
+  const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]), &ws = tensor(a[2]);
+  const int epi = (int)integer(a[4]);
+  Rows r;
+  MxRows v;
+  void* bias;
+  if (x.scalar_type() != kBf16 || !dense_rows(x, &r) || w.dim() != 2 || !mx_rows(w, ws, 16, &v) || v.K != r.K ||
+      x.device() != w.device() || !mx_bias(a[3], kBf16, v.M, x, &bias))
+    Py_RETURN_NONE;
+  const at::Tensor out = empty_like_rows(x, v.M, kBf16);
+  const int64_t head = (r.M * (r.K / 2) + 255) / 256 * 256;  // codes, and the scales behind them
+  const at::Tensor memory = empty({head + r.M * mx_scale_bytes(r.K)}, at::kByte, x);
+  uint8_t* const codes = static_cast<uint8_t*>(memory.data_ptr());
+  return with_status(status_of(x, lib.mxfp4_linear, x.data_ptr(), w.data_ptr(), ws.data_ptr(), bias, out.data_ptr(),
+                               codes, codes + head, r.M, v.M, r.K, r.ld, v.ld, v.lds, v.M, epi), {out});
+  END_HANDLE_TH_ERRORS
+}
+// w4a16(x, weight, weight_scale, bias, epilogue) -> (status, out)
+PyObject* w4a16(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 5);
+  const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]), &ws = tensor(a[2]);
+  const int epi = (int)integer(a[4]);
+  Rows r;
+  MxRows v;
+  void* bias;
+  if (x.scalar_type() != kBf16 || !dense_rows(x, &r) || w.dim() != 2 || !mx_rows(w, ws, 16, &v) || v.K != r.K ||
+      x.device() != w.device() || !mx_bias(a[3], kBf16, v.M, x, &bias))
+    Py_RETURN_NONE;
+  const at::Tensor out = empty_like_rows(x, v.M, kBf16);
+  return with_status(status_of(x, lib.w4a16_gemm, x.data_ptr(), w.data_ptr(), ws.data_ptr(), bias, out.data_ptr(), r.M,
+                               v.M, r.K, r.ld, v.ld, v.lds, v.M, epi), {out});
+  END_HANDLE_TH_ERRORS
+}
+
+// gate_residual_norm(x, branch, gate, shift, scale, norm_weight, post_weight, norm, post_norm, residual_scale, eps,
+// want_codes) -> (status, h, y), or (status, h, codes, scales)
+PyObject* gate_residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 12);
+  const at::Tensor &x = tensor(a[0]), &b = tensor(a[1]);
+  cdit_gate_residual_norm_args g = {};
+  Rows rx, rb;
+  g.x_dtype = dtype_id(x.scalar_type());
+  g.dtype = dtype_id(b.scalar_type());
+  const bool codes = a[11] == Py_True;
+  if (g.dtype < 0 || (g.x_dtype != g.dtype && g.x_dtype != CDIT_DT_F32) || x.sizes() != b.sizes() || x.dim() < 1 ||
+      !even_rows(x, &rx) || !even_rows(b, &rb) || rx.M <= 0 || rx.ld < rx.K || rb.ld < rb.K || b.device() != x.device() ||
+      (codes && rx.K % 32))
+    Py_RETURN_NONE;
+  g.M = rx.M;
+  g.K = rx.K;
+  bool any = false, plain = true;
+  // A vector of K, or one per index of x's first dimension, or one per row of x.
+  auto vec = [&](PyObject* o, const void** p, int64_t* ld, int64_t* rows_per) {
+    *p = nullptr;
+    if (o == Py_None || !plain) return;
+    const at::Tensor& t = tensor(o);
+    const int type = dtype_id(t.scalar_type());
+    const bool f32 = type == CDIT_DT_F32 && g.dtype != CDIT_DT_F32;
+    const int64_t d = t.dim(), count = g.K > 0 ? t.numel() / g.K : 0;
+    plain = d >= 1 && t.size(d - 1) == g.K && t.stride(d - 1) == 1 && (type == g.dtype || f32) && t.device() == x.device() &&
+            (!any || f32 == (g.vec_f32 != 0)) && count >= 1;
+    if (!plain) return;
+    any = true;
+    g.vec_f32 = f32;
+    *p = t.data_ptr();
+    if (count == 1) {
+      if (ld) {
+        *ld = 0;
+        *rows_per = g.M;
+      }
+      return;
+    }
+    if (!ld || g.M % count) {
+      plain = false;
+      return;
+    }
+    *rows_per = g.M / count;
+    if (x.dim() >= 2 && count == x.size(0) && t.size(0) == count) {
+      *ld = t.stride(0);
+    } else if (Rows rt; count == g.M && t.sizes() == x.sizes() && even_rows(t, &rt)) {
+      *ld = rt.ld;
+    } else {
+      plain = false;
+    }
+  };
+  vec(a[2], &g.gate, &g.ld_gate, &g.rows_per_gate);
+  vec(a[3], &g.shift, &g.ld_shift, &g.rows_per_shift);
+  vec(a[4], &g.scale, &g.ld_scale, &g.rows_per_scale);
+  vec(a[5], &g.norm_weight, nullptr, nullptr);
+  vec(a[6], &g.post_weight, nullptr, nullptr);
+  if (!plain) Py_RETURN_NONE;
+  g.norm = (int)integer(a[7]);
+  g.post_norm = (int)integer(a[8]);
+  g.residual_scale = (float)PyFloat_AsDouble(a[9]);
+  g.eps = (float)PyFloat_AsDouble(a[10]);
+  if (PyErr_Occurred()) throw python_error();
+  g.x = x.data_ptr();
+  g.ld_x = rx.ld;
+  g.branch = b.data_ptr();
+  g.ld_branch = rb.ld;
+  const at::Tensor h = empty(x.sizes(), x.scalar_type(), x);
+  g.h = h.data_ptr();
+  g.ld_h = g.K;
+  if (!codes) {
+    const at::Tensor y = empty(x.sizes(), b.scalar_type(), x);
+    g.y = y.data_ptr();
+    g.ld_y = g.K;
+    return with_status(status_of(x, lib.gate_residual_norm, &g), {h, y});
+  }
+  const at::Tensor q = empty_like_rows(x, g.K / 2, at::kByte), s = empty_like_rows(x, mx_scale_bytes(g.K), at::kByte);
+  g.codes = q.data_ptr();
+  g.ld_codes = g.K / 2;
+  g.code_scales = s.data_ptr();
+  g.ld_code_scales = mx_scale_bytes(g.K);
+  return with_status(status_of(x, lib.gate_residual_norm, &g), {h, q, s});
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(path): the library at `path`
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -620,6 +843,12 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   find(l.comm_per_token_dequant, "cdit_fp8_comm_per_token_dequant");
   find(l.comm_qkv_permute_quant, "cdit_fp8_comm_qkv_permute_quant");
   find(l.comm_qkv_permute_dequant, "cdit_fp8_comm_qkv_permute_dequant");
+  find(l.mxfp4_quant, "cdit_mxfp4_quant");
+  find(l.mxfp4_dequant, "cdit_mxfp4_dequant");
+  find(l.mxfp4_gemm, "cdit_mxfp4_gemm");
+  find(l.mxfp4_linear, "cdit_mxfp4_linear");
+  find(l.w4a16_gemm, "cdit_w4a16_gemm");
+  find(l.gate_residual_norm, "cdit_gate_residual_norm");
   lib = l;
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
@@ -647,6 +876,12 @@ PyMethodDef methods[] = {CDIT_METHOD(bind),
                          CDIT_METHOD(comm_per_token_dequant),
                          CDIT_METHOD(comm_qkv_permute_quant),
                          CDIT_METHOD(comm_qkv_permute_dequant),
+                         CDIT_METHOD(mxfp4_quant),
+                         CDIT_METHOD(mxfp4_dequant),
+                         CDIT_METHOD(mxfp4_mm),
+                         CDIT_METHOD(mxfp4_linear),
+                         CDIT_METHOD(w4a16),
+                         CDIT_METHOD(gate_residual_norm),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_cdit_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,144 @@
+// Device-side arithmetic of microscaled 4-bit floating point (OCP MX, E2M1 elements, one E8M0 scale
+// per 32 of them), shared by the quantizer, the GEMMs that read its codes and the block norm.
+#ifndef CDIT_MXFP4_DEVICE_H_
+#define CDIT_MXFP4_DEVICE_H_
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "cdit_internal.h"
+
+namespace cdit {
+namespace {
+
+constexpr int kMxBlock = 32;     // elements that share a scale
+constexpr int kMxNan = 255;      // scale byte of a block with a value that is not finite
+constexpr int kMxPad = 127;      // scale bytes behind the last block of a row: 2^0
+
+typedef __bf16 mx_v2bf __attribute__((ext_vector_type(2)));
+typedef _Float16 mx_v2h __attribute__((ext_vector_type(2)));
+typedef float mx_v2f __attribute__((ext_vector_type(2)));
+typedef unsigned int mx_v4u __attribute__((ext_vector_type(4)));
+typedef unsigned short mx_v2us __attribute__((ext_vector_type(2)));
+
+// The scale byte of a block from the fp32 bits of its largest magnitude: its exponent less 2, so that
+// the largest magnitude lands in [3.5, 7) of the element format, whose largest value is 6. Exponents
+// are counted after rounding up at a significand of 1.75: 7 and above would be cut to 6 (an error of
+// 1 and more in units of the scale); with the scale doubled it is rounded to 4, off by half at most. Never
+// below 1, which keeps 2^(e - 127) and its reciprocal normal fp32 numbers, nor above 252, so that no finite block
+// has a value beyond fp32 (magnitudes from 1.75 * 2^127 on are cut to 1.5 * 2^127); 255 (NaN) where the
+// magnitude is an infinity or a NaN: the element format has neither, and a block that hid them
+// would hand finite numbers on.
+__device__ __forceinline__ int mx_exponent(uint32_t amax_bits) {
+  const int e = (int)((amax_bits + 0x200000u) >> 23) - 2;
+  return amax_bits >= 0x7f800000u ? kMxNan : min(max(e, 1), 252);
+}
+
+// 2^(e - 127) as the converters take it: they read the exponent bits alone.
+__device__ __forceinline__ float mx_scale_f32(int e) { return __uint_as_float((uint32_t)e << 23); }
+
+// Eight consecutive elements as they lie in memory (four words of 16-bit types, eight of fp32).
+template <int DT>
+struct Mx8 {
+  uint32_t w[DT == CDIT_DT_F32 ? 8 : 4];
+};
+template <int DT>
+__device__ __forceinline__ Mx8<DT> mx_load8(const void* p) {
+  Mx8<DT> v;
+  const mx_v4u a = *reinterpret_cast<const mx_v4u*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.w[i] = a[i];
+  if constexpr (DT == CDIT_DT_F32) {
+    const mx_v4u b = *(reinterpret_cast<const mx_v4u*>(p) + 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.w[4 + i] = b[i];
+  }
+  return v;
+}
+// fp32 bits of the largest magnitude; an infinity or NaN gives 0x7f800000 or more.
+template <int DT>
+__device__ __forceinline__ uint32_t mx_amax8(const Mx8<DT>& v) {
+  if constexpr (DT == CDIT_DT_F32) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, v.w[i] & 0x7fffffffu);
+    return m;
+  } else {
+    mx_v2us m = {0, 0};  // magnitudes of 16-bit floats order like their bits
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(mx_v2us, v.w[i] & 0x7fff7fffu));
+    const uint32_t top = max((uint32_t)m[0], (uint32_t)m[1]);
+    if constexpr (DT == CDIT_DT_BF16) return top << 16;
+    return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)top));
+  }
+}
+// The largest of the four lanes of a quad, in all four: two DPP steps.
+__device__ __forceinline__ uint32_t mx_quad_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));  // quad_perm [1,0,3,2]
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));  // [2,3,0,1]
+}
+// Eight codes, element i in bits 4i .. 4i + 3: the hardware converters divide by the scale (exactly: it
+// is a power of two), round to the nearest code, ties to even, and cut to 6. A block with the NaN
+// scale has codes 0.
+template <int DT>
+__device__ __forceinline__ uint32_t mx_codes8(const Mx8<DT>& v, int e) {
+  if (e == kMxNan) return 0u;
+  const float s = mx_scale_f32(e);
+  uint32_t r = 0;
+  if constexpr (DT == CDIT_DT_F32) {
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(v.w[0]), __uint_as_float(v.w[1]), s, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(v.w[2]), __uint_as_float(v.w[3]), s, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(v.w[4]), __uint_as_float(v.w[5]), s, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(v.w[6]), __uint_as_float(v.w[7]), s, 3);
+  } else if constexpr (DT == CDIT_DT_BF16) {
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(mx_v2bf, v.w[0]), s, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(mx_v2bf, v.w[1]), s, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(mx_v2bf, v.w[2]), s, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(mx_v2bf, v.w[3]), s, 3);
+  } else {
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(mx_v2h, v.w[0]), s, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(mx_v2h, v.w[1]), s, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(mx_v2h, v.w[2]), s, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(mx_v2h, v.w[3]), s, 3);
+  }
+  return r;
+}
+// The values eight codes stand for, in the target type (bf16 and fp32: exact; fp16: rounded).
+template <int DT>
+__device__ __forceinline__ Mx8<DT> mx_values8(uint32_t c, int e) {
+  const float s = mx_scale_f32(e);
+  Mx8<DT> v;
+  if constexpr (DT == CDIT_DT_F32) {
+    const mx_v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
+    const mx_v2f d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2), f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
+    const float all[8] = {a[0], a[1], b[0], b[1], d[0], d[1], f[0], f[1]};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.w[i] = e == kMxNan ? 0x7fc00000u : __float_as_uint(all[i]);
+  } else if constexpr (DT == CDIT_DT_BF16) {
+    v.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0));
+    v.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1));
+    v.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2));
+    v.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.w[i] = e == kMxNan ? 0x7fc07fc0u : v.w[i];
+  } else {
+    v.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 0));
+    v.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 1));
+    v.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 2));
+    v.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 3));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.w[i] = e == kMxNan ? 0x7e007e00u : v.w[i];
+  }
+  return v;
+}
+template <int DT>
+__device__ __forceinline__ void mx_store8(void* p, const Mx8<DT>& v) {
+  *reinterpret_cast<mx_v4u*>(p) = mx_v4u{v.w[0], v.w[1], v.w[2], v.w[3]};
+  if constexpr (DT == CDIT_DT_F32)
+    *(reinterpret_cast<mx_v4u*>(p) + 1) = mx_v4u{v.w[4], v.w[5], v.w[6], v.w[7]};
+}
+
+}  // namespace
+}  // namespace cdit
+#endif

@@ -1,0 +1,112 @@
+// MXFP4 quantizer and its inverse (include/cdit_hip.h): both are bound by HBM.
+//
+// A lane takes 8 consecutive elements (16 bytes of a 16-bit type), so that a wavefront reads 1 KiB in a
+// row; the four lanes of a quad hold the 32 elements of a block, whose largest magnitude meets in two DPP
+// steps; the hardware converters do scaling and rounding. Nothing goes through LDS.
+#include "cdit_internal.h"
+#include "mxfp4_device.h"
+
+namespace cdit {
+namespace {
+
+constexpr int kThreads = 256;
+
+// Which rows a workgroup takes, so that short rows share one: a run of `rows`, walked as one line of
+// `rows * per_row` pieces of 8 elements. Piece -> row by a multiplication: magic = ceil(2^32 / per_row) is
+// exact while piece * per_row < 2^32 (at most 2^12 pieces where rows > 1, checked by the launcher).
+struct Runs {
+  int rows, per_row;
+  uint32_t magic;
+};
+Runs runs_of(int64_t K) {
+  const int per_row = (int)(K / 8);
+  const int rows = per_row >= 1024 ? 1 : 2048 / per_row;
+  return {rows, per_row, per_row == 1 ? 0u : (uint32_t)(((uint64_t(1) << 32) + per_row - 1) / per_row)};
+}
+__device__ __forceinline__ void locate(const Runs& r, uint32_t piece, uint32_t* row, uint32_t* at) {
+  *row = r.rows == 1 ? 0u : __umulhi(piece, r.magic);
+  *at = piece - *row * (uint32_t)r.per_row;
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void mxfp4_quant_rows(const uint8_t* __restrict__ x, int64_t ld_x,
+                                                             uint8_t* __restrict__ codes, int64_t ld_codes,
+                                                             uint8_t* __restrict__ scales, int64_t ld_scales,
+                                                             int64_t M, Runs r) {
+  constexpr int ES = DT == CDIT_DT_F32 ? 4 : 2;
+  const int64_t row0 = (int64_t)blockIdx.x * r.rows;
+  const uint32_t n = (uint32_t)min((int64_t)r.rows, M - row0) * (uint32_t)r.per_row;
+  const int blocks = r.per_row / 4;
+  for (uint32_t p = threadIdx.x; p < n; p += kThreads) {
+    uint32_t dr, at;
+    locate(r, p, &dr, &at);
+    const int64_t row = row0 + dr;
+    const Mx8<DT> v = mx_load8<DT>(x + (row * ld_x + (int64_t)at * 8) * ES);
+    // (per_row is a multiple of 4: a quad is in the row, and in the loop, as a whole)
+    const int e = mx_exponent(mx_quad_max(mx_amax8<DT>(v)));
+    *reinterpret_cast<uint32_t*>(codes + row * ld_codes + (int64_t)at * 4) = mx_codes8<DT>(v, e);
+    if (at % 4 == 0) {
+      uint8_t* const s = scales + row * ld_scales;
+      const int b = at / 4;
+      s[b] = (uint8_t)e;
+      if (b == blocks - 1)
+        for (int pad = blocks; pad % 4 != 0; ++pad) s[pad] = (uint8_t)kMxPad;
+    }
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void mxfp4_dequant_rows(const uint8_t* __restrict__ codes, int64_t ld_codes,
+                                                               const uint8_t* __restrict__ scales, int64_t ld_scales,
+                                                               uint8_t* __restrict__ out, int64_t ld_out, int64_t M,
+                                                               Runs r) {
+  constexpr int ES = DT == CDIT_DT_F32 ? 4 : 2;
+  const int64_t row0 = (int64_t)blockIdx.x * r.rows;
+  const uint32_t n = (uint32_t)min((int64_t)r.rows, M - row0) * (uint32_t)r.per_row;
+  for (uint32_t p = threadIdx.x; p < n; p += kThreads) {
+    uint32_t dr, at;
+    locate(r, p, &dr, &at);
+    const int64_t row = row0 + dr;
+    const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + row * ld_codes + (int64_t)at * 4);
+    const int e = scales[row * ld_scales + at / 4];
+    mx_store8<DT>(out + (row * ld_out + (int64_t)at * 8) * ES, mx_values8<DT>(c, e));
+  }
+}
+
+}  // namespace
+
+int launch_mxfp4_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ld_x, void* codes, int64_t ld_codes,
+                       void* scales, int64_t ld_scales, hipStream_t stream) {
+  const Runs r = runs_of(K);
+  const dim3 grid((unsigned)((M + r.rows - 1) / r.rows));
+#define CDIT_MXQ(DT)                                                                                        \
+  hipLaunchKernelGGL(mxfp4_quant_rows<DT>, grid, dim3(kThreads), 0, stream, static_cast<const uint8_t*>(x), \
+                     ld_x, static_cast<uint8_t*>(codes), ld_codes, static_cast<uint8_t*>(scales), ld_scales, M, r)
+  if (dtype == CDIT_DT_F32)
+    CDIT_MXQ(CDIT_DT_F32);
+  else if (dtype == CDIT_DT_BF16)
+    CDIT_MXQ(CDIT_DT_BF16);
+  else
+    CDIT_MXQ(CDIT_DT_F16);
+#undef CDIT_MXQ
+  return 0;
+}
+
+int launch_mxfp4_dequant(const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int64_t M, int64_t K,
+                         void* out, int dtype, int64_t ld_out, hipStream_t stream) {
+  const Runs r = runs_of(K);
+  const dim3 grid((unsigned)((M + r.rows - 1) / r.rows));
+#define CDIT_MXD(DT)                                                                                             \
+  hipLaunchKernelGGL(mxfp4_dequant_rows<DT>, grid, dim3(kThreads), 0, stream, static_cast<const uint8_t*>(codes), \
+                     ld_codes, static_cast<const uint8_t*>(scales), ld_scales, static_cast<uint8_t*>(out), ld_out, M, r)
+  if (dtype == CDIT_DT_F32)
+    CDIT_MXD(CDIT_DT_F32);
+  else if (dtype == CDIT_DT_BF16)
+    CDIT_MXD(CDIT_DT_BF16);
+  else
+    CDIT_MXD(CDIT_DT_F16);
+#undef CDIT_MXD
+  return 0;
+}
+
+}  // namespace cdit

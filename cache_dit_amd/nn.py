@@ -17,6 +17,7 @@ import torch
 from torch import nn
 
 from . import _native, ops
+from . import mxfp4  # (behind ops: each takes names of the other)
 from .logger import init_logger
 
 logger = init_logger(__name__)
@@ -41,30 +42,36 @@ def _note_inference_bypass(what: str) -> None:
 
 #: scale rounding used for activations and weights (see ops.fp8_rowwise_quant)
 DEFAULT_SCALE_MODE = "bf16div"
+_MXFP4_TYPES = ("mxfp4", "mxfp4_weight_only")
 
 
-def _quantize_weight(weight: torch.Tensor, scale_mode: str, per_tensor: bool = False):
-  """W bf16 [N,K] -> (codes e4m3 [N,K], scale fp32 [N,1]) with the HIP quantizer.
+def _quantize_weight(weight: torch.Tensor, scale_mode: str, quant_type: str):
+  """W bf16 [N,K] -> (codes e4m3 [N,K], scale fp32 [N,1]), or codes and block scales in MXFP4, with
+  the HIP quantizer.
 
   The reference quantizes the weight wherever it lives, and its CLI flow does so
   before `pipe.to(device)` (src/cache_dit/_utils/utils.py:2419,2459). There is no
   CPU kernel here, so a CPU weight makes a round trip through the GPU.
   """
   if weight.dtype != torch.bfloat16:
-    raise ValueError(f"weight must be bfloat16 to be quantized to FP8, got {weight.dtype}")
+    raise ValueError(f"weight must be bfloat16 to be quantized, got {weight.dtype}")
   src = weight.detach()
   if not src.is_cuda:
     if not torch.cuda.is_available():
       raise RuntimeError("quantizing a CPU weight needs a GPU to run the quantizer kernel on; "
                          "there is no CPU path")
     src = src.to("cuda")
-  quant = ops.fp8_tensorwise_quant if per_tensor else ops.fp8_rowwise_quant
-  q, s = quant(src.contiguous(), scale_mode)
+  if quant_type in _MXFP4_TYPES:
+    q, s = mxfp4.mxfp4_quant(src.contiguous())
+  else:
+    quant = ops.fp8_tensorwise_quant if quant_type == "float8_per_tensor" else ops.fp8_rowwise_quant
+    q, s = quant(src.contiguous(), scale_mode)
+    s = s.reshape(-1, 1).contiguous()
   return q.to(weight.device), s.to(weight.device)
 
 
 class _Fp8LinearBase(nn.Linear):
-  """Common state of the two quantized Linears. Never constructed directly:
+  """Common state of the quantized Linears. Never constructed directly:
   `convert_linear_` re-classes an existing nn.Linear."""
 
   weight_scale: torch.Tensor
@@ -294,10 +301,38 @@ class Fp8WeightOnlyLinear(_Fp8LinearBase):
                            self.epilogue)
 
 
+class Mxfp4Linear(_Fp8LinearBase):
+  """`mxfp4` (w4a4): weight and activation in microscaled 4-bit floating point, the activation
+  quantized per call; multiplied on the matrix cores as they are, fp32 sums, bias, optional
+  fused GELU-tanh, bf16 out. `weight` holds the codes uint8 [N, K/2], `weight_scale` the block
+  scales uint8 (layout: cache_dit_amd.mxfp4).
+
+  Also takes an activation that is in MXFP4 already, as the pair (codes, scales) of mxfp4_quant or
+  gate_residual_norm(quant_type="mxfp4"): siblings that read one activation quantize it once."""
+
+  def forward(self, x):
+    if isinstance(x, tuple):
+      codes, scales = x
+      return mxfp4.mxfp4_mm(codes, scales, self.weight, self.weight_scale, torch.bfloat16, self.bias, self.epilogue)
+    self._check_input(x)
+    return mxfp4.mxfp4_linear_op(x, self.weight, self.weight_scale, self.bias, self.epilogue)
+
+
+class Mxfp4WeightOnlyLinear(_Fp8LinearBase):
+  """`mxfp4_weight_only` (w4a16): bf16 activations, the weight in microscaled 4-bit floating
+  point, dequantized in the GEMM."""
+
+  def forward(self, x: torch.Tensor) -> torch.Tensor:
+    self._check_input(x)
+    return mxfp4.w4a16_mm_op(x, self.weight, self.weight_scale, self.bias, self.epilogue)
+
+
 _CLASS_OF = {
     "float8_per_row": Fp8DynamicLinear,
     "float8_per_tensor": Fp8DynamicLinearPerTensor,
     "float8_weight_only": Fp8WeightOnlyLinear,
+    "mxfp4": Mxfp4Linear,
+    "mxfp4_weight_only": Mxfp4WeightOnlyLinear,
 }
 
 
@@ -315,14 +350,17 @@ def convert_linear_(linear: nn.Linear,
     return linear
   if type(linear) is not nn.Linear and type(linear).forward is not nn.Linear.forward:
     raise TypeError(f"cannot convert {type(linear).__name__}: it overrides nn.Linear.forward")
-  if linear.in_features % 16 != 0 or linear.out_features % 16 != 0:
+  if quant_type in _MXFP4_TYPES:
+    if linear.in_features % 32 != 0:
+      raise ValueError(f"MXFP4 needs in features that are a multiple of 32, got {linear.in_features}")
+  elif linear.in_features % 16 != 0 or linear.out_features % 16 != 0:
     raise ValueError(f"FP8 matmul needs in/out features that are multiples of 16, got "
                      f"{linear.in_features}x{linear.out_features}")
-  q, s = _quantize_weight(linear.weight, scale_mode, per_tensor=quant_type == "float8_per_tensor")
+  q, s = _quantize_weight(linear.weight, scale_mode, quant_type)
   bias = linear.bias
   del linear.weight
   linear.weight = nn.Parameter(q, requires_grad=False)
-  linear.register_buffer("weight_scale", s.reshape(-1, 1).contiguous())
+  linear.register_buffer("weight_scale", s)
   if bias is not None:
     if bias.dtype != torch.bfloat16:
       raise ValueError(f"bias must be bfloat16, got {bias.dtype}")
@@ -576,4 +614,6 @@ def linear_on_cat(linear: nn.Module, xs) -> torch.Tensor:
 
 def dequantize_weight(linear: _Fp8LinearBase) -> torch.Tensor:
   """bf16 view of the quantized weight (for inspection and tests)."""
+  if linear.quant_type in _MXFP4_TYPES:
+    return mxfp4.mxfp4_dequant(linear.weight, linear.weight_scale)
   return (linear.weight.to(torch.float32) * linear.weight_scale).to(torch.bfloat16)

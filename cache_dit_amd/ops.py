@@ -975,3 +975,8 @@ def w8a16_mm(x: torch.Tensor,
              epilogue: int = 0) -> torch.Tensor:
   _require_cuda("w8a16_mm", x, b_data)
   return w8a16_mm_op(x, b_data, b_scale, bias, encode_output_dtype(output_dtype), epilogue)
+
+
+# The 4-bit operators and the block norm (their module takes its helpers from this one).
+from .mxfp4 import (gate_residual_norm, mxfp4_dequant, mxfp4_linear, mxfp4_mm,  # noqa: E402,F401
+                    mxfp4_quant, w4a16_mm)

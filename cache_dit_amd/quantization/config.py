@@ -14,7 +14,8 @@ from typing import Any, Callable, Dict, List, Optional, Union
 
 from .backend import QuantizeBackend
 
-#: quant types the reference's online path accepts (quantize_ao.py:16-27)
+#: quant types the reference's online path accepts (quantize_ao.py:16-27), and in the place of its nvfp4
+#: types, which are another vendor's format, the microscaled 4-bit format of this hardware
 ALLOWED_QUANTIZE_TYPES = [
     "float8_per_row",
     "float8_per_tensor",
@@ -22,13 +23,15 @@ ALLOWED_QUANTIZE_TYPES = [
     "float8_weight_only",
     "nvfp4",
     "nvfp4_weight_only",
+    "mxfp4",
+    "mxfp4_weight_only",
     "int8_per_row",
     "int8_per_tensor",
     "int8_weight_only",
     "int4_weight_only",
 ]
 #: the ones with MI355X kernels behind them
-BUILT_QUANTIZE_TYPES = ["float8_per_row", "float8_per_tensor", "float8_weight_only"]
+BUILT_QUANTIZE_TYPES = ["float8_per_row", "float8_per_tensor", "float8_weight_only", "mxfp4", "mxfp4_weight_only"]
 
 _DEFAULT_EXCLUDE = ("embedder", "embed", "modulation", "mod")
 

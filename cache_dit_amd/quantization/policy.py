@@ -33,6 +33,8 @@ PRECISION_PLAN_ORDER = [
     "float8_weight_only",
     "nvfp4",
     "nvfp4_weight_only",
+    "mxfp4",
+    "mxfp4_weight_only",
     "int8_per_tensor",
     "int8_per_row",
     "int8_weight_only",
@@ -174,6 +176,9 @@ class QuantizeContext:
   def is_float8(self) -> bool:
     return "float8" in self.quant_type
 
+  def is_mxfp4(self) -> bool:
+    return "mxfp4" in self.quant_type
+
   def is_weight_only(self) -> bool:
     return "weight_only" in self.quant_type
 
@@ -313,7 +318,7 @@ def basic_filter(m: nn.Module, name: str, ctx: QuantizeContext,
     if shape[-2] % 128 != 0 or shape[-1] % 128 != 0:
       return skip(f"w{shape} % blocksize(128, 128) != 0")
 
-  if qt in ("float8_per_row", "float8_per_tensor", "float8_per_block") and not _bias_ok(m):
+  if qt in ("float8_per_row", "float8_per_tensor", "float8_per_block", "mxfp4", "mxfp4_weight_only") and not _bias_ok(m):
     return skip("_scaled_mm: DTensor + bias NOT supported")
 
   incompatible = _kernel_incompatibility(m, qt)
@@ -352,15 +357,19 @@ def fallback_filter(m: nn.Module, name: str, ctx: QuantizeContext) -> bool:
 
 
 def _kernel_incompatibility(m: nn.Linear, qt: str) -> Optional[str]:
-  """Why the FP8 kernels cannot take Linear `m` under quant type `qt` (None if they
+  """Why the kernels cannot take Linear `m` under quant type `qt` (None if they
   can). The reference hands every layer to torchao, whose FP8 configs leave a layer
   they cannot run unquantized without raising; here such a layer is skipped with a
   reason before anything about it is recorded, for every quant type that has a
-  kernel: both weight dimensions multiples of 16, bf16 weight and bias."""
+  kernel: both weight dimensions multiples of 16 (MXFP4: in_features a multiple of 32,
+  whole blocks), bf16 weight and bias."""
   if qt not in BUILT_QUANTIZE_TYPES:
     return None
   shape = tuple(m.weight.shape)
-  if shape[-2] % 16 != 0 or shape[-1] % 16 != 0:
+  if "mxfp4" in qt:
+    if shape[-1] % 32 != 0:
+      return f"weight_shape{shape}[-1]%32!=0"
+  elif shape[-2] % 16 != 0 or shape[-1] % 16 != 0:
     return f"weight_shape{shape}%16!=0"
   if m.weight.dtype != torch.bfloat16:
     return f"dtype({m.weight.dtype})!=bfloat16"
@@ -421,6 +430,7 @@ def _check_platform(ctx: QuantizeContext) -> None:
   if ctx.is_float8():
     cap = torch.cuda.get_device_capability()
     assert cap >= (8, 9), f"FP8 requires a GPU with FP8 matrix cores, but got capability {cap}"
+  if ctx.is_float8() or ctx.is_mxfp4():
     _native.device_arch()  # raises unless the device is a gfx950
 
 

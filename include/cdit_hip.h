@@ -356,6 +356,109 @@ int cdit_fp8_linear_w8a8_static(const void* x_bf16, const void* w_q, const float
                                 int scale_mode, int epilogue, int out_dtype_id, void* stream);
 
 /*
+ * Microscaled 4-bit floating point (MXFP4: OCP MX, E2M1 elements with one E8M0 scale per 32 of them along K), the
+ * format the matrix cores of gfx950 take as it is. It stands where the reference's block-scaled 4-bit types stand
+ * ("nvfp4", "nvfp4_weight_only", src/cache_dit/quantization/torchao/quantize_ao.py:16-27), which are another
+ * vendor's format.
+ *
+ * codes  uint8 [M, K/2]: element 2j in the low half of byte j, 2j + 1 in the high half; bit 3 the sign, bits 0..2 the
+ *        magnitude 0, .5, 1, 1.5, 2, 3, 4, 6.
+ * scales uint8 [M, 4 ceil(K/128)]: byte b is the scale 2^(s - 127) of elements 32 b .. 32 b + 31, 255 a NaN; the up to
+ *        three bytes behind K/32 are 127. (For K a multiple of 128 that is [M, K/32] without padding.)
+ * K is a multiple of 32. Leading dimensions of codes and scales are in bytes; rows of codes start on a multiple of 4
+ * bytes for the quantizer and its inverse, of 16 for the GEMMs; rows of scales on a multiple of 4.
+ *
+ * cdit_mxfp4_quant: x [M,K] (ld_x in elements, rows on 16 bytes) of x_dtype_id ->
+ *   amax = max over a block of |x|
+ *   s    = the exponent of amax (as fp32 stores it; one more where its significand is 1.75 or more) less 2, in 1 .. 252;
+ *          255 where the block holds an infinity or a NaN
+ *   code = the nearest value to x 2^(127 - s), ties to the even code, at most 6 in magnitude; 0 where s is 255
+ * cdit_mxfp4_dequant: out [M,K] (ld_out in elements, rows on 16 bytes) = value * 2^(s - 127) in out_dtype_id (bf16 and
+ *   fp32 exact; fp16 rounded, to infinity where it overflows), NaN where s is 255.
+ */
+int cdit_mxfp4_quant(const void* x, int x_dtype_id, int64_t M, int64_t K, int64_t ld_x, void* codes, int64_t ld_codes,
+                     void* scales, int64_t ld_scales, void* stream);
+int cdit_mxfp4_dequant(const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int64_t M, int64_t K,
+                       void* out, int out_dtype_id, int64_t ld_out, void* stream);
+
+/*
+ * GEMM on MXFP4 operands (w4a4) with fused epilogue:
+ *   out[m,n] = epi( sum_k a[m,k] b[n,k] + bias[n] )
+ * a: codes [M,K/2] and scales (as above), b: the weight's [N,K/2] and scales; out [M,N] (ldo in elements) of
+ * out_dtype_id; bias [N] of the output's dtype or NULL. Sums are held in fp32 by the matrix instruction. Any N, any ldo.
+ */
+int cdit_mxfp4_gemm(const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales, const void* bias,
+                    void* out, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldas, int64_t ldb, int64_t ldbs,
+                    int64_t ldo, int epilogue, int out_dtype_id, void* stream);
+
+/*
+ * One Linear forward in that mode: cdit_mxfp4_quant of x (bf16 [M,K], ld_x) into the caller's workspaces (codes_ws
+ * M * K/2 bytes, scales_ws M * 4 ceil(K/128) bytes, both on 16 bytes), then cdit_mxfp4_gemm; out and bias bf16.
+ */
+int cdit_mxfp4_linear(const void* x_bf16, const void* w_codes, const void* w_scales, const void* bias_bf16, void* out,
+                      void* codes_ws, void* scales_ws, int64_t M, int64_t N, int64_t K, int64_t ld_x, int64_t ldw,
+                      int64_t ldws, int64_t ldo, int epilogue, void* stream);
+
+/*
+ * Weight-only GEMM with an MXFP4 weight (w4a16): x bf16 [M,K] (lda in elements, rows on 16 bytes), the weight's codes
+ * and scales as above, bias bf16 [N] or NULL, out bf16 [M,N] (ldo in elements). The weight's values are exact in
+ * bf16; products are summed in fp32. Any N, any ldo.
+ */
+int cdit_w4a16_gemm(const void* x_bf16, const void* w_codes, const void* w_scales, const void* bias_bf16, void* out,
+                    int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldw, int64_t ldws, int64_t ldo, int epilogue,
+                    void* stream);
+
+/*
+ * What stands between two branches of a block: the branch's own norm (sandwich norms), its gate, the scaled residual
+ * sum, the next norm and its modulation, in one pass over the activation. In a DiT block the sequence
+ * `hidden = hidden + gate * attn_output; norm2(hidden) * (1 + scale) + shift` of the blocks whose forwards the
+ * reference patches (src/cache_dit/caching/patch_functors/functor_flux.py:48-80); with weights in place of the
+ * modulation, the residual path of a language model. Per row m:
+ *
+ *   t = branch[m], or norm_post(branch[m]) [* post_weight]
+ *   h = residual_scale x[m] + [gate *] t
+ *   y = norm(h) [* norm_weight] [* (1 + scale)] [+ shift]
+ *   norm(v) = (v - mean v) / sqrt(mean (v - mean v)^2 + eps)   CDIT_NORM_LAYER
+ *           = v / sqrt(mean v^2 + eps)                         CDIT_NORM_RMS
+ *
+ * in fp32 throughout; h and y are rounded once, where they are stored, and y comes from the unrounded h. x and h have
+ * x_dtype, branch and y have dtype; x_dtype is dtype or fp32 (a residual stream held in fp32). gate, shift, scale,
+ * norm_weight and post_weight have dtype, or all of them fp32 (vec_f32); NULL: left out. Row m takes vector m /
+ * rows_per_* of gate, shift and scale (ld_* elements apart). y or codes may be NULL: with codes (K a multiple of 32) the
+ * MXFP4 codes and scales of y, rounded to dtype first, are written (as cdit_mxfp4_quant writes them).
+ * Any K, stride and alignment is taken; h and y must not overlap the inputs.
+ */
+enum cdit_norm { CDIT_NORM_NONE = 0, CDIT_NORM_LAYER = 1, CDIT_NORM_RMS = 2 };
+typedef struct cdit_gate_residual_norm_args {
+  int64_t M, K;
+  const void* x;
+  int64_t ld_x;
+  const void* branch;
+  int64_t ld_branch;
+  int x_dtype, dtype;
+  const void* gate;
+  int64_t ld_gate, rows_per_gate;
+  const void* shift;
+  int64_t ld_shift, rows_per_shift;
+  const void* scale;
+  int64_t ld_scale, rows_per_scale;
+  const void* norm_weight;
+  const void* post_weight;
+  int vec_f32;
+  int norm, post_norm; /* CDIT_NORM_LAYER or _RMS; post_norm may be _NONE */
+  float residual_scale, eps;
+  void* h;
+  int64_t ld_h;
+  void* y;
+  int64_t ld_y;
+  void* codes;
+  int64_t ld_codes;
+  void* code_scales;
+  int64_t ld_code_scales;
+} cdit_gate_residual_norm_args;
+int cdit_gate_residual_norm(const cdit_gate_residual_norm_args* args, void* stream);
+
+/*
  * Writes to *id the id of the graph capture that `stream` is recording into, 0 when it is
  * not capturing. For bindings that keep per-stream state between calls (the Python
  * binding reuses activation codes across sibling Linears): state made inside one capture
