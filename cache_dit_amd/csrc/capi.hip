@@ -747,7 +747,7 @@ int cdit_mxfp4_gemm(const void* a_codes, const void* a_scales, const void* b_cod
   const Mx4Gemm g{static_cast<const uint8_t*>(a_codes), static_cast<const uint8_t*>(a_scales),
                   static_cast<const uint8_t*>(b_codes), static_cast<const uint8_t*>(b_scales), bias, out, (int)M, (int)N,
                   (int)K, lda, ldas, ldb, ldbs, ldo, epilogue, out_dtype_id};
-  rc = launch_gemm_mxfp4(g, static_cast<hipStream_t>(stream));
+  rc = launch_gemm_mxfp4(g, g_gemm_variant, static_cast<hipStream_t>(stream));
   return rc ? rc : after_launch(fn);
 }
 
@@ -774,7 +774,7 @@ int cdit_w4a16_gemm(const void* x_bf16, const void* w_codes, const void* w_scale
   const Mx4Gemm g{static_cast<const uint8_t*>(x_bf16), nullptr, static_cast<const uint8_t*>(w_codes),
                   static_cast<const uint8_t*>(w_scales), bias_bf16, out, (int)M, (int)N, (int)K, lda, 0, ldw, ldws, ldo,
                   epilogue, CDIT_DT_BF16};
-  rc = launch_gemm_w4a16(g, static_cast<hipStream_t>(stream));
+  rc = launch_gemm_w4a16(g, g_gemm_variant, static_cast<hipStream_t>(stream));
   return rc ? rc : after_launch(fn);
 }
 

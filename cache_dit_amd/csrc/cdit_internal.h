@@ -138,8 +138,9 @@ struct Mx4Gemm {
   int64_t lda, ldas, ldb, ldbs, ldo;  // a: bytes (w4a4) or elements (w4a16); ldo: elements; the others bytes
   int epilogue, out_dtype;
 };
-int launch_gemm_mxfp4(const Mx4Gemm& g, hipStream_t stream);
-int launch_gemm_w4a16(const Mx4Gemm& g, hipStream_t stream);
+// variant < 0: choose by shape.
+int launch_gemm_mxfp4(const Mx4Gemm& g, int variant, hipStream_t stream);
+int launch_gemm_w4a16(const Mx4Gemm& g, int variant, hipStream_t stream);
 
 // What stands between two branches of a block (block_norm.hip); the arguments are checked by the caller.
 int launch_gate_residual_norm(const cdit_gate_residual_norm_args& a, hipStream_t stream);

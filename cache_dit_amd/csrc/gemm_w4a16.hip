@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void gemm_w4a16_direct(Mx4Gemm g) {
 
 }  // namespace
 
-int launch_gemm_w4a16(const Mx4Gemm& g, hipStream_t stream) {
+int launch_gemm_w4a16(const Mx4Gemm& g, int variant, hipStream_t stream) {
   const dim3 grid((unsigned)((g.N + 127) / 128), (unsigned)((g.M + 31) / 32));
   hipLaunchKernelGGL(gemm_w4a16_direct, grid, dim3(256), 0, stream, g);
   return 0;
