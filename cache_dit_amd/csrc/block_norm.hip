@@ -131,10 +131,12 @@ struct Row {
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = (t[i] - mean) * rstd * (a.post_weight ? w[i] : 1.0f);
   }
-  // t -> h
-  __device__ __forceinline__ void residual(int c, float (&t)[8]) const {
-    float x[8], g[8];
+  __device__ __forceinline__ void stream(int c, float (&x)[8]) const {
     load8<ST, VEC>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + 8 * c) * size_of<ST>(), n_of(c), x);
+  }
+  // t, x -> h
+  __device__ __forceinline__ void residual(int c, const float (&x)[8], float (&t)[8]) const {
+    float g[8];
     if (a.gate) vec(a.gate, a.ld_gate, a.rows_per_gate, c, g);
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = __fmaf_rn(a.gate ? g[i] : 1.0f, t[i], a.residual_scale * x[i]);
@@ -229,7 +231,9 @@ __global__ __launch_bounds__(256) void gate_residual_norm_any(Args a) {
     auto h_of = [&](int c, float(&f)[8]) {
       r.branch(c, f);
       if (a.post_norm) r.post(c, pm, pr, f);
-      r.residual(c, f);
+      float x[8];
+      r.stream(c, x);
+      r.residual(c, x, f);
     };
     statistics(a, a.norm == CDIT_NORM_LAYER, sum, threadIdx.x, 256, pieces, h_of, &mean, &rstd);
     for (int c = threadIdx.x; c < pieces; c += 256) {
@@ -240,8 +244,124 @@ __global__ __launch_bounds__(256) void gate_residual_norm_any(Args a) {
   }
 }
 
+// The row in registers: CH pieces per lane, WAVES wavefronts per row, 16-byte accesses. A workgroup takes a run of consecutive
+// rows; the next row's loads are under way while a row is worked on.
+template <int ST, int DT, int WAVES, int CH>
+__global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, int rows_per_wg) {
+  __shared__ float slots[2][WAVES];
+  BlockSum<WAVES> sum{slots, 0};
+  const int64_t row0 = (int64_t)blockIdx.x * rows_per_wg, row_end = min(a.M, row0 + rows_per_wg);
+  const float inv_k = 1.0f / (float)a.K;
+  Mx8<DT> b_raw[2][CH];
+  Mx8<ST> x_raw[2][CH];
+  auto piece = [&](int c) { return (c * WAVES + (int)(threadIdx.x >> 6)) * 64 + (int)(threadIdx.x & 63); };
+  auto fetch = [&](int64_t row, Mx8<DT>(&bb)[CH], Mx8<ST>(&xx)[CH]) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      bb[c] = {};
+      xx[c] = {};
+      if (8 * piece(c) < a.K) {
+        bb[c] = mx_load8<DT>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + 8 * piece(c)) * size_of<DT>());
+        xx[c] = mx_load8<ST>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + 8 * piece(c)) * size_of<ST>());
+      }
+    }
+  };
+  // mean and 1 / sqrt(...) of the row whose pieces are f, as in statistics()
+  auto stats = [&](const float(&f)[CH][8], bool layer, float* mean, float* rstd) {
+    float s = 0.0f;
+    *mean = 0.0f;
+    if (layer) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += f[c][i];  // (pieces behind the row are zeros)
+      *mean = sum(s) * inv_k;
+      s = 0.0f;
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const bool in = 8 * piece(c) < a.K;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = in ? f[c][i] - *mean : 0.0f;
+        s = __fmaf_rn(d, d, s);
+      }
+    }
+    *rstd = 1.0f / __fsqrt_rn(sum(s) * inv_k + a.eps);
+  };
+  auto one_row = [&](int64_t row, Mx8<DT>(&bb)[CH], Mx8<ST>(&xx)[CH], Mx8<DT>(&nb)[CH], Mx8<ST>(&nx)[CH]) {
+    if (row + 1 < row_end) fetch(row + 1, nb, nx);
+    const Row<ST, DT, true> r{a, row};
+    float h[CH][8], mean, rstd;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) widen8<DT>(bb[c], h[c]);
+    if (a.post_norm) {
+      stats(h, a.post_norm == CDIT_NORM_LAYER, &mean, &rstd);
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (8 * piece(c) < a.K) r.post(piece(c), mean, rstd, h[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float x[8];
+      widen8<ST>(xx[c], x);
+      if (8 * piece(c) < a.K) r.residual(piece(c), x, h[c]);
+    }
+    stats(h, a.norm == CDIT_NORM_LAYER, &mean, &rstd);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (8 * piece(c) < a.K) r.finish(piece(c), mean, rstd, h[c]);
+  };
+  if (row0 >= row_end) return;
+  fetch(row0, b_raw[0], x_raw[0]);
+  for (int64_t row = row0; row < row_end; row += 2) {
+    one_row(row, b_raw[0], x_raw[0], b_raw[1], x_raw[1]);
+    if (row + 1 < row_end) one_row(row + 1, b_raw[1], x_raw[1], b_raw[0], x_raw[0]);
+  }
+}
+
+template <int ST, int DT>
+bool rows_fit(const Args& a) {
+  constexpr int SS = size_of<ST>(), DS = size_of<DT>();
+  auto rows = [](const void* p, int64_t ld, int size) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0;
+  };
+  const int vs = a.vec_f32 ? 4 : DS;
+  auto vec = [&](const void* p, int64_t ld) { return !p || rows(p, ld, vs); };
+  return a.K % 8 == 0 && a.K <= 16384 && rows(a.x, a.ld_x, SS) && rows(a.h, a.ld_h, SS) && rows(a.branch, a.ld_branch, DS) &&
+         (!a.y || rows(a.y, a.ld_y, DS)) && vec(a.gate, a.ld_gate) && vec(a.shift, a.ld_shift) && vec(a.scale, a.ld_scale) &&
+         vec(a.norm_weight, 0) && vec(a.post_weight, 0);
+}
+
 template <int ST, int DT>
 int launch_types(const Args& a, hipStream_t stream) {
+  if (rows_fit<ST, DT>(a)) {
+    const int cus = cu_count();
+    if (cus <= 0) {
+      set_error("cannot query the CU count of the current device");
+      return CDIT_EHIP;
+    }
+    const int pieces = (int)(a.K / 8);
+#define CDIT_NORM_CASE(W, CH)                                                                                         \
+  if (pieces <= 64 * W * CH) {                                                                                        \
+    const int64_t target = (int64_t)cus * std::max(1, 24 / W);                                                        \
+    const int per = (int)std::min<int64_t>((a.M + target - 1) / target, 1 << 20);                                     \
+    hipLaunchKernelGGL((gate_residual_norm_rows<ST, DT, W, CH>), dim3((unsigned)((a.M + per - 1) / per)), dim3(64 * W), 0, \
+                       stream, a, per);                                                                               \
+    return 0;                                                                                                         \
+  }
+    CDIT_NORM_CASE(1, 1)
+    CDIT_NORM_CASE(1, 2)
+    CDIT_NORM_CASE(2, 2)
+    CDIT_NORM_CASE(3, 2)
+    CDIT_NORM_CASE(4, 2)
+    CDIT_NORM_CASE(5, 2)
+    CDIT_NORM_CASE(6, 2)
+    CDIT_NORM_CASE(8, 2)
+    CDIT_NORM_CASE(12, 2)
+    CDIT_NORM_CASE(16, 2)
+#undef CDIT_NORM_CASE
+  }
   const dim3 grid((unsigned)std::min<int64_t>(a.M, 1 << 20));
   hipLaunchKernelGGL((gate_residual_norm_any<ST, DT>), grid, dim3(256), 0, stream, a);
   return 0;

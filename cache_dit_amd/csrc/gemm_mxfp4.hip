@@ -386,7 +386,7 @@ gemm_mxfp4_tile(Mx4Gemm g, int tiles_m, int tiles_n) {
     const uint32_t off_out = (uint32_t)(wm * WM + 4 * h) * row_bytes + (uint32_t)n * OB;
     const bool whole = g.N % TN == 0 && g.ldo % TN == 0 && reinterpret_cast<uintptr_t>(g.out) % (TN * OB) == 0;
     constexpr int kStoreOnce = 2;  // non-temporal: whole lines, written once
-    auto store_tile = [&](auto gelu_tag) {
+    auto store_tile = [&](auto gelu_tag, auto whole_tag) {
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -398,7 +398,7 @@ gemm_mxfp4_tile(Mx4Gemm g, int tiles_m, int tiles_n) {
             v[j] = acc[i][j][e];
             if constexpr (decltype(gelu_tag)::value) v[j] = gelu_tanh(v[j]);
           }
-          if (whole) {
+          if constexpr (decltype(whole_tag)::value) {
             const int at = (int)(n < g.N ? off_out : 0x80000000u);
             if constexpr (OUT == CDIT_DT_F32) {
               if constexpr (TN == 4)
@@ -431,10 +431,15 @@ gemm_mxfp4_tile(Mx4Gemm g, int tiles_m, int tiles_n) {
           }
         }
     };
-    if (g.epilogue & CDIT_EPI_GELU_TANH)
-      store_tile(std::true_type{});
+    const bool gelu = (g.epilogue & CDIT_EPI_GELU_TANH) != 0;
+    if (whole && gelu)
+      store_tile(std::true_type{}, std::true_type{});
+    else if (whole)
+      store_tile(std::false_type{}, std::true_type{});
+    else if (gelu)
+      store_tile(std::true_type{}, std::false_type{});
     else
-      store_tile(std::false_type{});
+      store_tile(std::false_type{}, std::false_type{});
     if (!more) break;
     cur = nxt;
   }
