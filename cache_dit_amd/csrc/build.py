@@ -18,7 +18,7 @@ LIB_DIR = os.path.join(os.path.dirname(HERE), "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libcdit_hip.so")
 HOST_PATH = os.path.join(LIB_DIR, "_cdit_host.so")
 SOURCES = ["capi.hip", "quant_rowwise.hip", "comm_quant.hip", "gemm_fp8.hip", "gemm_w8a16.hip",
-           "mxfp4_quant.hip", "gemm_mxfp4.hip", "gemm_w4a16.hip", "block_norm.hip"]
+           "mxfp4_quant.hip", "gemm_mxfp4.hip", "gemm_mx_rows.hip", "gemm_w4a16.hip", "block_norm.hip"]
 
 # -ffp-contract=off: the quantizer's arithmetic is specified operation by
 # operation (explicit FMAs only). The packed-fp32 feature is switched off on

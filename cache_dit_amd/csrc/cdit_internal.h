@@ -141,6 +141,11 @@ struct Mx4Gemm {
 // variant < 0: choose by shape.
 int launch_gemm_mxfp4(const Mx4Gemm& g, int variant, hipStream_t stream);
 int launch_gemm_w4a16(const Mx4Gemm& g, int variant, hipStream_t stream);
+// Up to 16 rows (gemm_mx_rows.hip). The Linear: g.a is the bf16 activation, g.lda in elements; the kernel quantizes it.
+bool mx_rows_fit(int M);
+int launch_gemm_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream);
+int launch_linear_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream);
+int launch_gemm_w4a16_rows(const Mx4Gemm& g, hipStream_t stream);
 
 // What stands between two branches of a block (block_norm.hip); the arguments are checked by the caller.
 int launch_gate_residual_norm(const cdit_gate_residual_norm_args& a, hipStream_t stream);

@@ -1,0 +1,238 @@
+// The 4-bit Linears for up to 16 rows (single tokens, conditioning vectors): a stream of weights.
+//
+// A workgroup takes G times 16 output columns. The activation goes to LDS first (in pieces of K where it is long), and is
+// quantized on the way where the caller has it in bf16. K is split between the W wavefronts in items of 512; a wavefront reads an
+// item's weights straight from memory (every byte is used once, the next item's loads are under way meanwhile) and multiplies
+// them with the activation's rows on the matrix core, and the W partial sums of 16 x 16 outputs meet in LDS. Bound by HBM, and
+// by latency where N is small.
+//
+// Lane l is row l & 15 (a column of the output; a row of the activation) and K block l >> 4 of a step of 128: 16 bytes of codes,
+// 64 of each row in a request, and the scale in byte l >> 4 of the step's word. The scales go through LDS: 16 rows of them are
+// a few KB in a row, fetched by the whole workgroup at once. (A word per lane and item straight from memory, whether 16
+// bytes of each row or 256 in a row, held a loop of nothing but the loads to 4.1 TB/s where the codes alone ran at 5.2.)
+#include <algorithm>
+
+#include "gemm_common.h"
+#include "mxfp4_device.h"
+
+namespace cdit {
+namespace {
+
+// Weight-only: bf16 activation. Codes: an activation in MXFP4. Quantize: a bf16 activation, quantized here.
+enum Mode { kWeightOnly, kCodes, kQuantize };
+constexpr int kItem = 512;            // along K
+constexpr int kMostWaves = 8;
+constexpr int kMostLds = 64 * 1024;   // of activation: two workgroups fit a CU
+
+// Bytes of a row of the activation in LDS for `items` items, and of a row of scales. 16 (4) more than a multiple of 256 (16): the
+// 16 rows a pass reads start in different banks.
+__host__ __device__ constexpr int row_pitch(int mode, int items) { return items * (mode == kWeightOnly ? 1024 : 256) + 16; }
+__host__ __device__ constexpr int scale_pitch(int items) { return items * 16 + 4; }
+
+template <int MODE, int OUT>
+__global__ __launch_bounds__(64 * kMostWaves) void gemm_mx_rows(Mx4Gemm g, int G, int chunk_items) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int r = lane & 15, kg = lane >> 4;
+  const int KB = g.K / kMxBlock, S = (g.K + 127) / 128 * 4, items = (g.K + kItem - 1) / kItem;
+  const int pitch = row_pitch(MODE, chunk_items), spitch = MODE == kWeightOnly ? 0 : scale_pitch(chunk_items);
+  float* const part = reinterpret_cast<float*>(smem);  // [G][waves][256]
+  uint8_t* const wscale = smem + G * waves * 1024;  // [16 G][wpitch]
+  const int wpitch = scale_pitch(chunk_items);
+  uint8_t* const xs = wscale + 16 * G * wpitch;
+  uint8_t* const xe = xs + g.M * pitch;
+  const int m = min(r, g.M - 1);  // (rows that do not exist repeat the last: their results are not stored)
+
+  struct Weights {
+    v4u c[4];
+  };
+  // (buffer accesses: what lies behind K, and rows behind the last, read as zeros without a branch around the load)
+  auto load = [&](int group, int item, Weights& w) {
+    const int n0 = 16 * (blockIdx.x * G + group), rows = min(g.N - n0, 16);
+    const __amdgpu_buffer_rsrc_t codes = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(g.b + (int64_t)n0 * g.ldb), 0, rows > 0 ? (rows - 1) * (int)g.ldb + g.K / 2 : 0, 0x00020000);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int block = 16 * item + 4 * s + kg;
+      const int at = (int)(block < KB ? (uint32_t)r * (uint32_t)g.ldb + 16u * block : 0x80000000u);
+      w.c[s] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(codes, at, 0, 0));
+    }
+  };
+  auto multiply = [&](const Weights& w, int group, int in_chunk, v4f (&acc)[2]) {
+    const uint8_t* const ws = wscale + (16 * group + r) * wpitch + 16 * in_chunk + kg;
+    const uint8_t* const x = xs + m * pitch + in_chunk * (MODE == kWeightOnly ? 1024 : 256) + kg * (MODE == kWeightOnly ? 64 : 16);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int e = ws[4 * s];
+      if constexpr (MODE == kWeightOnly) {
+        const float f = e == kMxNan ? __uint_as_float(0x7fc00000u) : mx_scale_f32(e);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          acc[q & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_to_bf16(w.c[s][q], f),
+                                                               *reinterpret_cast<const v8bf*>(x + 256 * s + 16 * q), acc[q & 1], 0, 0, 0);
+      } else {
+        const v4i c = __builtin_bit_cast(v4i, w.c[s]), a = *reinterpret_cast<const v4i*>(x + 64 * s);
+        const v8i w8 = __builtin_shufflevector(c, c, 0, 1, 2, 3, -1, -1, -1, -1);
+        const v8i x8 = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
+        const int xe_s = xe[m * spitch + 16 * in_chunk + 4 * s + kg];
+        acc[s & 1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[s & 1], 4, 4, 0, e, 0, xe_s);
+      }
+    }
+  };
+
+  for (int i = threadIdx.x; i < G * waves * 256; i += blockDim.x) part[i] = 0.0f;
+  for (int first = 0; first < items; first += chunk_items) {
+    const int n_items = min(chunk_items, items - first), per = (n_items + waves - 1) / waves;
+    // this wavefront's items of the chunk, for each group of columns; the first two items' weights go out before the activation
+    const int mine = min(max(n_items - wave * per, 0), per), i0 = first + wave * per;
+    Weights w[2];
+    int lg = 0, li = 0;  // group and item to load next
+    auto load_next = [&](Weights& into) {
+      if (lg >= G || mine <= 0) return;
+      load(lg, i0 + li, into);
+      if (++li == mine) {
+        li = 0;
+        ++lg;
+      }
+    };
+    // Blocks of the activation and words of the weight's scales, a thread's first of each before the weights: a wait for a load
+    // is a wait for all before it.
+    struct Block {
+      Mx8<CDIT_DT_BF16> v[4];  // (codes: v[0], and the scale)
+      int e;
+    };
+    const int n_blocks = 16 * n_items, n_words = 4 * n_items;
+    auto fetch_block = [&](int t) -> Block {
+      Block x = {};
+      const int row = t / n_blocks, block = 16 * first + t - row * n_blocks;
+      x.e = kMxPad;
+      if (block >= KB) return x;
+      if constexpr (MODE == kCodes) {
+        x.v[0] = mx_load8<CDIT_DT_BF16>(g.a + (int64_t)row * g.lda + 16 * block);
+        x.e = g.a_scale[(int64_t)row * g.ldas + block];
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x.v[q] = mx_load8<CDIT_DT_BF16>(g.a + 2 * ((int64_t)row * g.lda + 32 * block + 8 * q));
+      }
+      return x;
+    };
+    auto put_block = [&](int t, const Block& x) {
+      const int row = t / n_blocks, b = t - row * n_blocks;
+      if constexpr (MODE == kWeightOnly) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mx_store8<CDIT_DT_BF16>(xs + row * pitch + 64 * b + 16 * q, x.v[q]);
+      } else if constexpr (MODE == kCodes) {
+        mx_store8<CDIT_DT_BF16>(xs + row * pitch + 16 * b, x.v[0]);
+        xe[row * spitch + b] = (uint8_t)x.e;
+      } else {
+        uint32_t top = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) top = max(top, mx_amax8<CDIT_DT_BF16>(x.v[q]));
+        const int e = mx_exponent(top);
+        v4u c;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) c[q] = mx_codes8<CDIT_DT_BF16>(x.v[q], e);
+        *reinterpret_cast<v4u*>(xs + row * pitch + 16 * b) = c;
+        xe[row * spitch + b] = (uint8_t)e;
+      }
+    };
+    auto fetch_word = [&](int t) -> uint32_t {  // words behind a row's last: the scales of zeros
+      const int row = t / n_words, word = t - row * n_words, at = 16 * first + 4 * word;
+      const int64_t n = min(16 * (int)blockIdx.x * G + row, g.N - 1);
+      return at < S ? *reinterpret_cast<const uint32_t*>(g.b_scale + n * g.ldbs + at) : 0x7f7f7f7fu;
+    };
+    auto put_word = [&](int t, uint32_t v) {
+      const int row = t / n_words;
+      *reinterpret_cast<uint32_t*>(wscale + row * wpitch + 4 * (t - row * n_words)) = v;
+    };
+    const int blocks = g.M * n_blocks, words = 16 * G * n_words, t0 = threadIdx.x;
+    Block x0 = {};
+    uint32_t v0 = 0;
+    if (t0 < blocks) x0 = fetch_block(t0);
+    if (t0 < words) v0 = fetch_word(t0);
+    load_next(w[0]);
+    load_next(w[1]);
+    if (first > 0) __syncthreads();  // the piece before has been read
+    if (t0 < blocks) put_block(t0, x0);
+    if (t0 < words) put_word(t0, v0);
+    for (int t = t0 + blockDim.x; t < blocks; t += blockDim.x) put_block(t, fetch_block(t));
+    for (int t = t0 + blockDim.x; t < words; t += blockDim.x) put_word(t, fetch_word(t));
+    __syncthreads();
+    v4f acc[2] = {};
+    int group = 0, i = 0;  // of the item at hand
+    auto one_item = [&](Weights& now) {
+      const bool last = i + 1 == mine;
+      multiply(now, group, i0 + i - first, acc);
+      load_next(now);
+      if (last) {  // (a lane's own place: what an earlier piece of K left there is its own)
+        v4f* const p = reinterpret_cast<v4f*>(part + (group * waves + wave) * 256 + 4 * lane);
+        *p = *p + (acc[0] + acc[1]);
+        acc[0] = acc[1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        ++group;
+        i = 0;
+      } else {
+        ++i;
+      }
+    };
+    if (mine > 0) {
+      while (true) {
+        one_item(w[0]);
+        if (group == G) break;
+        one_item(w[1]);
+        if (group == G) break;
+      }
+    }
+  }
+  __syncthreads();
+  // element e of lane l: column 4 (l >> 4) + e, row l & 15
+  for (int t = threadIdx.x; t < G * 16 * g.M; t += blockDim.x) {
+    const int c = t % (16 * G), row = t / (16 * G), n = 16 * blockIdx.x * G + c;
+    if (n >= g.N) continue;
+    const float* const p = part + (c >> 4) * waves * 256 + 4 * (16 * ((c & 15) >> 2) + row) + (c & 3);
+    float v = 0.0f;
+    for (int k = 0; k < waves; ++k) v += p[256 * k];
+    store_mx_one<OUT>(g, row, n, v);
+  }
+}
+
+template <int MODE, int OUT>
+int launch_rows(const Mx4Gemm& g, hipStream_t stream) {
+  static bool lds_allowed[64];
+  const int cus = cu_count();
+  if (cus <= 0) {
+    set_error("cannot query the CU count of the current device");
+    return CDIT_EHIP;
+  }
+  const int items = std::max(1, (g.K + kItem - 1) / kItem), groups = (g.N + 15) / 16;
+  // as many items of activation as fit; even shares of them for the wavefronts
+  int chunk = items;
+  while (chunk > 1 && g.M * (row_pitch(MODE, chunk) + scale_pitch(chunk)) > kMostLds) --chunk;
+  const int per = (chunk + kMostWaves - 1) / kMostWaves, waves = (chunk + per - 1) / per;
+  // Two groups of columns a workgroup where there are more than two for each CU: 30720 columns, K 5120, one row 23.1 us with one,
+  // 21.5 with two, 23.9 with four (5 wavefronts; 10 are slower throughout). 8 wavefronts at most: 13824 columns, K 5120
+  // 12.8 us with 5 or 8, 15.6 with 10; K 16384 33.2 with 8, 41.1 with 16.
+  const int G = groups > 2 * cus ? 2 : 1;
+  const int lds = G * waves * 1024 + 16 * G * scale_pitch(chunk) + g.M * (row_pitch(MODE, chunk) + scale_pitch(chunk));
+  if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&gemm_mx_rows<MODE, OUT>), 160 * 1024, lds_allowed)) return rc;
+  hipLaunchKernelGGL((gemm_mx_rows<MODE, OUT>), dim3((unsigned)((groups + G - 1) / G)), dim3(64 * waves), lds, stream, g, G,
+                     chunk);
+  return 0;
+}
+template <int MODE>
+int launch_rows(const Mx4Gemm& g, hipStream_t stream) {
+  switch (g.out_dtype) {
+    case CDIT_DT_F16: return launch_rows<MODE, CDIT_DT_F16>(g, stream);
+    case CDIT_DT_F32: return launch_rows<MODE, CDIT_DT_F32>(g, stream);
+    default: return launch_rows<MODE, CDIT_DT_BF16>(g, stream);
+  }
+}
+
+}  // namespace
+
+bool mx_rows_fit(int M) { return M >= 1 && M <= 16; }
+
+int launch_gemm_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream) { return launch_rows<kCodes>(g, stream); }
+int launch_linear_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream) { return launch_rows<kQuantize, CDIT_DT_BF16>(g, stream); }
+int launch_gemm_w4a16_rows(const Mx4Gemm& g, hipStream_t stream) { return launch_rows<kWeightOnly, CDIT_DT_BF16>(g, stream); }
+
+}  // namespace cdit

@@ -17,22 +17,6 @@ __device__ __forceinline__ v4f mfma_mx(v4i w, v4i a, v4f acc, int w_scale, int a
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, a8, acc, 4, 4, 0, w_scale, 0, a_scale);
 }
 
-// One element of the output from its sum.
-template <int OUT>
-__device__ __forceinline__ void store_one(const Mx4Gemm& g, int m, int n, float v) {
-  if (g.bias) v += OUT == CDIT_DT_F32 ? static_cast<const float*>(g.bias)[n]
-                                      : bias_to_f32<OUT>(static_cast<const uint16_t*>(g.bias)[n]);
-  if (g.epilogue & CDIT_EPI_GELU_TANH) v = gelu_tanh(v);
-  const int64_t at = (int64_t)m * g.ldo + n;
-  if constexpr (OUT == CDIT_DT_F32) {
-    static_cast<float*>(g.out)[at] = v;
-  } else if constexpr (OUT == CDIT_DT_F16) {
-    static_cast<uint16_t*>(g.out)[at] = __builtin_bit_cast(uint16_t, (_Float16)v);
-  } else {
-    static_cast<uint16_t*>(g.out)[at] = (uint16_t)f32_to_bf16_bits(v);
-  }
-}
-
 // A wavefront per 32 x 32 outputs, operands straight from memory.
 template <int OUT>
 __global__ __launch_bounds__(256) void gemm_mxfp4_direct(Mx4Gemm g) {
@@ -73,7 +57,7 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_direct(Mx4Gemm g) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int m = m0 + 16 * i + r, n = n0 + 16 * j + 4 * kg + e;
-        if (m < g.M && n < g.N) store_one<OUT>(g, m, n, acc[i][j][e]);
+        if (m < g.M && n < g.N) store_mx_one<OUT>(g, m, n, acc[i][j][e]);
       }
 }
 
@@ -472,6 +456,7 @@ int launch_tile(const Mx4Gemm& g, hipStream_t stream) {
 }  // namespace
 
 int launch_gemm_mxfp4(const Mx4Gemm& g, int variant, hipStream_t stream) {
+  if (variant < 0 && mx_rows_fit(g.M)) return launch_gemm_mxfp4_rows(g, stream);
   // (offsets inside a tile are 32 bits)
   const bool small_strides = std::max({g.lda, g.ldas, g.ldb, g.ldbs, 4 * g.ldo}) * 256 < INT32_MAX;
   if (variant < 0 && g.M > 32 && small_strides) {

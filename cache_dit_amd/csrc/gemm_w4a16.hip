@@ -9,12 +9,6 @@
 namespace cdit {
 namespace {
 
-// Eight codes as bf16, times their scale.
-__device__ __forceinline__ v8bf mx_to_bf16(uint32_t c, float scale) {
-  const v2bf c0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0), c1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1);
-  const v2bf c2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2), c3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3);
-  return v8bf{c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
-}
 // The scale of a block as the converter takes it; NaN for a NaN block.
 __device__ __forceinline__ float mx_weight_scale(int e) { return e == kMxNan ? __uint_as_float(0x7fc00000u) : mx_scale_f32(e); }
 
@@ -75,6 +69,7 @@ __global__ __launch_bounds__(256) void gemm_w4a16_direct(Mx4Gemm g) {
 }  // namespace
 
 int launch_gemm_w4a16(const Mx4Gemm& g, int variant, hipStream_t stream) {
+  if (variant < 0 && mx_rows_fit(g.M)) return launch_gemm_w4a16_rows(g, stream);
   const dim3 grid((unsigned)((g.N + 127) / 128), (unsigned)((g.M + 31) / 32));
   hipLaunchKernelGGL(gemm_w4a16_direct, grid, dim3(256), 0, stream, g);
   return 0;

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include "cdit_internal.h"
+#include "gemm_common.h"
 
 namespace cdit {
 namespace {
@@ -137,6 +138,28 @@ __device__ __forceinline__ void mx_store8(void* p, const Mx8<DT>& v) {
   *reinterpret_cast<mx_v4u*>(p) = mx_v4u{v.w[0], v.w[1], v.w[2], v.w[3]};
   if constexpr (DT == CDIT_DT_F32)
     *(reinterpret_cast<mx_v4u*>(p) + 1) = mx_v4u{v.w[4], v.w[5], v.w[6], v.w[7]};
+}
+
+// Eight codes as bf16, times their scale.
+__device__ __forceinline__ v8bf mx_to_bf16(uint32_t c, float scale) {
+  const v2bf c0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0), c1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1);
+  const v2bf c2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2), c3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3);
+  return v8bf{c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
+}
+// One element of the output from its sum.
+template <int OUT>
+__device__ __forceinline__ void store_mx_one(const Mx4Gemm& g, int m, int n, float v) {
+  if (g.bias) v += OUT == CDIT_DT_F32 ? static_cast<const float*>(g.bias)[n]
+                                      : bias_to_f32<OUT>(static_cast<const uint16_t*>(g.bias)[n]);
+  if (g.epilogue & CDIT_EPI_GELU_TANH) v = gelu_tanh(v);
+  const int64_t at = (int64_t)m * g.ldo + n;
+  if constexpr (OUT == CDIT_DT_F32) {
+    static_cast<float*>(g.out)[at] = v;
+  } else if constexpr (OUT == CDIT_DT_F16) {
+    static_cast<uint16_t*>(g.out)[at] = __builtin_bit_cast(uint16_t, (_Float16)v);
+  } else {
+    static_cast<uint16_t*>(g.out)[at] = (uint16_t)f32_to_bf16_bits(v);
+  }
 }
 
 }  // namespace
