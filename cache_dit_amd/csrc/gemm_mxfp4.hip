@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "gemm_common.h"
+#include "mx_tile.h"
 #include "mxfp4_device.h"
 
 namespace cdit {
@@ -126,7 +127,6 @@ gemm_mxfp4_tile(Mx4Gemm g, int tiles_m, int tiles_n) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   constexpr int TM = C::TM, TN = C::TN, MF = TM * TN, SA = C::SA, SB = C::SB, NDA = C::NDA, NDB = C::NDB;
   constexpr int WAVES = C::WAVES, WM = C::WM, WN = C::WN;
-  constexpr int OB = OUT == CDIT_DT_F32 ? 4 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WGN, wn = wave % C::WGN, r32 = lane & 31, h = lane >> 5;
   const int KB = g.K / kMxBlock, KT = max((g.K + 255) / 256, C::MIN_STEPS), S = (g.K + 127) / 128 * 4;
@@ -241,19 +241,8 @@ gemm_mxfp4_tile(Mx4Gemm g, int tiles_m, int tiles_n) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) sb[j] = order_scales(b_raw[j]);
   };
-  // the bias of this lane's columns; columns that do not exist: 0
   float bias[TN];
-  auto load_bias = [&](const Source& s) {
-    const int n = s.n0 + wn * WN + TN * r32;
-    const __amdgpu_buffer_rsrc_t buf = buffer(static_cast<const uint8_t*>(g.bias), g.bias ? g.N * OB : 0);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      if constexpr (OUT == CDIT_DT_F32)
-        bias[j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, (n + j) * OB, 0, 0));
-      else
-        bias[j] = bias_to_f32<OUT>((uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(buf, (n + j) * OB, 0, 0));
-    }
-  };
+  auto load_bias = [&](const Source& s) { mx_bias<TN, OUT>(g, s.n0 + wn * WN + TN * r32, bias); };
 
   Source cur = source_of(blockIdx.x), nxt = cur;
   load_scales(cur, 0);
@@ -361,69 +350,7 @@ gemm_mxfp4_tile(Mx4Gemm g, int tiles_m, int tiles_n) {
     const bool more = tile + (int)gridDim.x < ntiles;
     if (more) load_bias(nxt);
 
-    // Out: element e of a block is row 8 (e >> 2) + 4 h + (e & 3). A lane's TN columns are one store, 32 lanes a row of the
-    // wavefront's tile.
-    const int rows = min(C::BM, g.M - cur.m0), n = cur.n0 + wn * WN + TN * r32;
-    const int64_t out0 = (int64_t)cur.m0 * g.ldo * OB;
-    const __amdgpu_buffer_rsrc_t out = buffer(static_cast<const uint8_t*>(g.out) + out0, ((rows - 1) * (int)g.ldo + g.N) * OB);
-    const uint32_t row_bytes = (uint32_t)g.ldo * OB;
-    const uint32_t off_out = (uint32_t)(wm * WM + 4 * h) * row_bytes + (uint32_t)n * OB;
-    const bool whole = g.N % TN == 0 && g.ldo % TN == 0 && reinterpret_cast<uintptr_t>(g.out) % (TN * OB) == 0;
-    constexpr int kStoreOnce = 2;  // non-temporal: whole lines, written once
-    auto store_tile = [&](auto gelu_tag, auto whole_tag) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint32_t row = (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3)) * row_bytes;
-          float v[TN];
-#pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            v[j] = acc[i][j][e];
-            if constexpr (decltype(gelu_tag)::value) v[j] = gelu_tanh(v[j]);
-          }
-          if constexpr (decltype(whole_tag)::value) {
-            const int at = (int)(n < g.N ? off_out : 0x80000000u);
-            if constexpr (OUT == CDIT_DT_F32) {
-              if constexpr (TN == 4)
-                __builtin_amdgcn_raw_buffer_store_b128(
-                    v4u{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}, out, at,
-                    row, kStoreOnce);
-              else if constexpr (TN == 2)
-                __builtin_amdgcn_raw_buffer_store_b64(v2u{__float_as_uint(v[0]), __float_as_uint(v[1])}, out, at, row, kStoreOnce);
-              else
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[0]), out, at, row, kStoreOnce);
-            } else {
-              auto pack = [](float lo, float hi) { return OUT == CDIT_DT_F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); };
-              if constexpr (TN == 4)
-                __builtin_amdgcn_raw_buffer_store_b64(v2u{pack(v[0], v[1]), pack(v[2], v[3])}, out, at, row, kStoreOnce);
-              else if constexpr (TN == 2)
-                __builtin_amdgcn_raw_buffer_store_b32(pack(v[0], v[1]), out, at, row, kStoreOnce);
-              else
-                __builtin_amdgcn_raw_buffer_store_b16((short)pack(v[0], 0.0f), out, at, row, kStoreOnce);
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < TN; ++j) {
-              const int at = (int)(n + j < g.N ? off_out + j * OB : 0x80000000u);
-              if constexpr (OUT == CDIT_DT_F32)
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[j]), out, at, row, 0);
-              else
-                __builtin_amdgcn_raw_buffer_store_b16(
-                    (short)(OUT == CDIT_DT_F16 ? pack_f16x2(v[j], 0.0f) : pack_bf16x2(v[j], 0.0f)), out, at, row, 0);
-            }
-          }
-        }
-    };
-    const bool gelu = (g.epilogue & CDIT_EPI_GELU_TANH) != 0;
-    if (whole && gelu)
-      store_tile(std::true_type{}, std::true_type{});
-    else if (whole)
-      store_tile(std::false_type{}, std::true_type{});
-    else if (gelu)
-      store_tile(std::true_type{}, std::false_type{});
-    else
-      store_tile(std::false_type{}, std::false_type{});
+    store_mx_tile<TM, TN, OUT>(acc, g, cur.m0, C::BM, wm * WM + 4 * h, cur.n0 + wn * WN + TN * r32);
     if (!more) break;
     cur = nxt;
   }

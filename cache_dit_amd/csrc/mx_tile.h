@@ -1,0 +1,110 @@
+// What the tiles of the two 4-bit GEMMs share: both hold their outputs as blocks of 32 x 32 in the layout of the 32-row matrix
+// instructions, a lane (r32 = lane & 31, h = lane >> 5) TN consecutive columns n .. n + TN - 1 of the rows 32 i + 8 (e >> 2) + 4 h
+// + (e & 3).
+#ifndef CDIT_MX_TILE_H_
+#define CDIT_MX_TILE_H_
+
+#include <type_traits>
+
+#include "gemm_common.h"
+
+namespace cdit {
+namespace {
+
+// The bias of a lane's columns in fp32; 0 for columns that do not exist, and without a bias.
+template <int TN, int OUT>
+__device__ __forceinline__ void mx_bias(const Mx4Gemm& g, int n, float (&bias)[TN]) {
+  constexpr int OB = OUT == CDIT_DT_F32 ? 4 : 2;
+  const __amdgpu_buffer_rsrc_t buf =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(g.bias), 0, g.bias ? g.N * OB : 0, 0x00020000);
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    if constexpr (OUT == CDIT_DT_F32)
+      bias[j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, (n + j) * OB, 0, 0));
+    else
+      bias[j] = bias_to_f32<OUT>((uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(buf, (n + j) * OB, 0, 0));
+  }
+}
+
+// Stores a wavefront's blocks from the registers they are in: a lane's TN columns are one store, 32 lanes a whole row of the
+// wavefront's tile. The tile's rows are m0 .. m0 + bm - 1, row: this lane's first inside it.
+template <int TM, int TN, int OUT>
+__device__ __forceinline__ void store_mx_tile(v16f (&acc)[TM][TN], const Mx4Gemm& g, int m0, int bm, int row, int n) {
+  constexpr int OB = OUT == CDIT_DT_F32 ? 4 : 2;
+  const int rows = min(bm, g.M - m0);
+  const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
+      static_cast<uint8_t*>(g.out) + (int64_t)m0 * g.ldo * OB, 0, ((rows - 1) * (int)g.ldo + g.N) * OB, 0x00020000);
+  const uint32_t row_bytes = (uint32_t)g.ldo * OB;
+  const uint32_t off = (uint32_t)row * row_bytes + (uint32_t)n * OB;
+  const bool whole = g.N % TN == 0 && g.ldo % TN == 0 && reinterpret_cast<uintptr_t>(g.out) % (TN * OB) == 0;
+  constexpr int kStoreOnce = 2;  // non-temporal: whole lines, written once
+  auto store = [&](auto gelu_tag, auto whole_tag) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t at_row = (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3)) * row_bytes;
+        float v[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          v[j] = acc[i][j][e];
+          if constexpr (decltype(gelu_tag)::value) v[j] = gelu_tanh(v[j]);
+        }
+        auto pack = [](float lo, float hi) -> uint32_t {
+          return OUT == CDIT_DT_F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+        };
+        if constexpr (decltype(whole_tag)::value) {
+          const int at = (int)(n < g.N ? off : 0x80000000u);
+          if constexpr (OUT == CDIT_DT_F32) {
+            uint32_t w[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) w[j] = __float_as_uint(v[j]);
+            if constexpr (TN == 4) {
+              const v4u d = {w[0], w[1], w[2], w[3]};
+              __builtin_amdgcn_raw_buffer_store_b128(d, out, at, at_row, kStoreOnce);
+            } else if constexpr (TN == 2) {
+              const v2u d = {w[0], w[1]};
+              __builtin_amdgcn_raw_buffer_store_b64(d, out, at, at_row, kStoreOnce);
+            } else {
+              const uint32_t d = w[0];
+              __builtin_amdgcn_raw_buffer_store_b32(d, out, at, at_row, kStoreOnce);
+            }
+          } else if constexpr (TN == 4) {
+            const v2u d = {pack(v[0], v[1]), pack(v[2], v[3])};
+            __builtin_amdgcn_raw_buffer_store_b64(d, out, at, at_row, kStoreOnce);
+          } else if constexpr (TN == 2) {
+            const uint32_t d = pack(v[0], v[1]);
+            __builtin_amdgcn_raw_buffer_store_b32(d, out, at, at_row, kStoreOnce);
+          } else {
+            const short d = (short)pack(v[0], 0.0f);
+            __builtin_amdgcn_raw_buffer_store_b16(d, out, at, at_row, kStoreOnce);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const int at = (int)(n + j < g.N ? off + j * OB : 0x80000000u);
+            if constexpr (OUT == CDIT_DT_F32) {
+              const uint32_t d = __float_as_uint(v[j]);
+              __builtin_amdgcn_raw_buffer_store_b32(d, out, at, at_row, 0);
+            } else {
+              const short d = (short)pack(v[j], 0.0f);
+              __builtin_amdgcn_raw_buffer_store_b16(d, out, at, at_row, 0);
+            }
+          }
+        }
+      }
+  };
+  const bool gelu = (g.epilogue & CDIT_EPI_GELU_TANH) != 0;
+  if (whole && gelu)
+    store(std::true_type{}, std::true_type{});
+  else if (whole)
+    store(std::false_type{}, std::true_type{});
+  else if (gelu)
+    store(std::true_type{}, std::false_type{});
+  else
+    store(std::false_type{}, std::false_type{});
+}
+
+}  // namespace
+}  // namespace cdit
+#endif
