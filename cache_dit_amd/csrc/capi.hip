@@ -757,7 +757,7 @@ int cdit_mxfp4_linear(const void* x_bf16, const void* w_codes, const void* w_sca
   const char* fn = "cdit_mxfp4_linear";
   int rc = check_mx_gemm(fn, w_codes, w_scales, out, M, N, K, ldw, ldws, ldo, epilogue, CDIT_DT_BF16);
   if (rc || (rc = check_mx(fn, "the workspaces", codes_ws, scales_ws, M, K, K / 2, mx_scale_bytes(K), 16))) return rc;
-  if (g_gemm_variant < 0 && mx_rows_fit((int)M) && N > 0) {  // few rows: one kernel that quantizes them itself
+  if (g_gemm_variant < 0 && N > 0 && mx_rows_fit(false, (int)M, (int)N)) {  // few rows: one kernel that quantizes them itself
     if ((rc = check_mx_dense(fn, x_bf16, M, K, ld_x, CDIT_DT_BF16)) || (rc = check_arch())) return rc;
     const Mx4Gemm g{static_cast<const uint8_t*>(x_bf16), nullptr, static_cast<const uint8_t*>(w_codes),
                     static_cast<const uint8_t*>(w_scales), bias_bf16, out, (int)M, (int)N, (int)K, ld_x, 0, ldw, ldws, ldo,

@@ -141,8 +141,12 @@ struct Mx4Gemm {
 // variant < 0: choose by shape.
 int launch_gemm_mxfp4(const Mx4Gemm& g, int variant, hipStream_t stream);
 int launch_gemm_w4a16(const Mx4Gemm& g, int variant, hipStream_t stream);
+// What the automatic choice runs: 0 the kernel without tiles, 1 .. the tiles, kMxRows the kernel for few rows.
+constexpr int kMxRows = 100;
+int choose_gemm_mxfp4(const Mx4Gemm& g);
+int choose_gemm_w4a16(const Mx4Gemm& g);
 // Up to 16 rows (gemm_mx_rows.hip). The Linear: g.a is the bf16 activation, g.lda in elements; the kernel quantizes it.
-bool mx_rows_fit(int M);
+bool mx_rows_fit(bool weight_only, int M, int N);
 int launch_gemm_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream);
 int launch_linear_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream);
 int launch_gemm_w4a16_rows(const Mx4Gemm& g, hipStream_t stream);

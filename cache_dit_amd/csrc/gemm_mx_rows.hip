@@ -22,7 +22,7 @@ namespace {
 enum Mode { kWeightOnly, kCodes, kQuantize };
 constexpr int kItem = 512;            // along K
 constexpr int kMostWaves = 8;
-constexpr int kMostLds = 64 * 1024;   // of activation: two workgroups fit a CU
+constexpr int kMostLds = 64 * 1024;   // of activation and scales: two workgroups fit a CU
 
 // Bytes of a row of the activation in LDS for `items` items, and of a row of scales. 16 (4) more than a multiple of 256 (16): the
 // 16 rows a pass reads start in different banks.
@@ -204,15 +204,16 @@ int launch_rows(const Mx4Gemm& g, hipStream_t stream) {
     return CDIT_EHIP;
   }
   const int items = std::max(1, (g.K + kItem - 1) / kItem), groups = (g.N + 15) / 16;
-  // as many items of activation as fit; even shares of them for the wavefronts
-  int chunk = items;
-  while (chunk > 1 && g.M * (row_pitch(MODE, chunk) + scale_pitch(chunk)) > kMostLds) --chunk;
-  const int per = (chunk + kMostWaves - 1) / kMostWaves, waves = (chunk + per - 1) / per;
   // Two groups of columns a workgroup where there are more than two for each CU: 30720 columns, K 5120, one row 23.1 us with one,
   // 21.5 with two, 23.9 with four (5 wavefronts; 10 are slower throughout). 8 wavefronts at most: 13824 columns, K 5120
   // 12.8 us with 5 or 8, 15.6 with 10; K 16384 33.2 with 8, 41.1 with 16.
   const int G = groups > 2 * cus ? 2 : 1;
-  const int lds = G * waves * 1024 + 16 * G * scale_pitch(chunk) + g.M * (row_pitch(MODE, chunk) + scale_pitch(chunk));
+  // as many items of the activation and of scales as fit; even shares of them for the wavefronts
+  auto bytes = [&](int n) { return g.M * (row_pitch(MODE, n) + scale_pitch(n)) + 16 * G * scale_pitch(n); };
+  int chunk = items;
+  while (chunk > 1 && bytes(chunk) > kMostLds) --chunk;
+  const int per = (chunk + kMostWaves - 1) / kMostWaves, waves = (chunk + per - 1) / per;
+  const int lds = G * waves * 1024 + bytes(chunk);
   if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&gemm_mx_rows<MODE, OUT>), 160 * 1024, lds_allowed)) return rc;
   hipLaunchKernelGGL((gemm_mx_rows<MODE, OUT>), dim3((unsigned)((groups + G - 1) / G)), dim3(64 * waves), lds, stream, g, G,
                      chunk);
@@ -229,7 +230,13 @@ int launch_rows(const Mx4Gemm& g, hipStream_t stream) {
 
 }  // namespace
 
-bool mx_rows_fit(int M) { return M >= 1 && M <= 16; }
+// Whether this is the kernel for so many rows and columns, and not a tile. Every workgroup handles the whole activation, so its
+// time grows with rows times columns; us, this kernel and the best tile (w4a4 with its quantizer), M x N x K, weights from HBM:
+// w4a4 4 x 13824 x 5120 14.9 and 18.1, 8: 17.1 and 18.5, 16: 21.2 and 18.2; 16 x 5120 x 5120 14.0 and 14.8; 16 x 30720 x 5120 38.8
+// and 25.5. Weight-only 8 x 13824 x 5120 17.9 and 24.4, 16: 23.7 and 25.1; 16 x 30720 x 5120 45.9 and 32.4.
+bool mx_rows_fit(bool weight_only, int M, int N) {
+  return M >= 1 && M <= 16 && (int64_t)M * ((N + 15) / 16) < (weight_only ? 20000 : 10000);
+}
 
 int launch_gemm_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream) { return launch_rows<kCodes>(g, stream); }
 int launch_linear_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream) { return launch_rows<kQuantize, CDIT_DT_BF16>(g, stream); }

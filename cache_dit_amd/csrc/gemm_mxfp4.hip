@@ -22,44 +22,46 @@ __device__ __forceinline__ v4f mfma_mx(v4i w, v4i a, v4f acc, int w_scale, int a
 template <int OUT>
 __global__ __launch_bounds__(256) void gemm_mxfp4_direct(Mx4Gemm g) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
-  const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 128 + wave * 32;
+  const int n0 = blockIdx.x * 128 + wave * 32;
   if (n0 >= g.N) return;
   const int blocks = g.K / kMxBlock, steps = (g.K + 127) / 128;
-  const uint8_t *a[2], *as[2], *w[2], *ws[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t m = min(m0 + 16 * i + r, g.M - 1), n = min(n0 + 16 * i + r, g.N - 1);
-    a[i] = g.a + m * g.lda + 16 * kg;
-    as[i] = g.a_scale + m * g.ldas + kg;
-    w[i] = g.b + n * g.ldb + 16 * kg;
-    ws[i] = g.b_scale + n * g.ldbs + kg;
-  }
-  v4f acc[2][2] = {};
-  for (int s = 0; s < steps; ++s) {
-    const bool in = 4 * s + kg < blocks;  // codes behind K count as zeros; the scale rows are padded
-    v4i av[2], wv[2];
-    int asv[2], wsv[2];
+  for (int m0 = blockIdx.y * 32; m0 < g.M; m0 += gridDim.y * 32) {
+    const uint8_t *a[2], *as[2], *w[2], *ws[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      av[i] = in ? *reinterpret_cast<const v4i*>(a[i] + 64 * (int64_t)s) : v4i{0, 0, 0, 0};
-      wv[i] = in ? *reinterpret_cast<const v4i*>(w[i] + 64 * (int64_t)s) : v4i{0, 0, 0, 0};
-      asv[i] = as[i][4 * s];
-      wsv[i] = ws[i][4 * s];
+      const int64_t m = min(m0 + 16 * i + r, g.M - 1), n = min(n0 + 16 * i + r, g.N - 1);
+      a[i] = g.a + m * g.lda + 16 * kg;
+      as[i] = g.a_scale + m * g.ldas + kg;
+      w[i] = g.b + n * g.ldb + 16 * kg;
+      ws[i] = g.b_scale + n * g.ldbs + kg;
+    }
+    v4f acc[2][2] = {};
+    for (int s = 0; s < steps; ++s) {
+      const bool in = 4 * s + kg < blocks;  // codes behind K count as zeros; the scale rows are padded
+      v4i av[2], wv[2];
+      int asv[2], wsv[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        av[i] = in ? *reinterpret_cast<const v4i*>(a[i] + 64 * (int64_t)s) : v4i{0, 0, 0, 0};
+        wv[i] = in ? *reinterpret_cast<const v4i*>(w[i] + 64 * (int64_t)s) : v4i{0, 0, 0, 0};
+        asv[i] = as[i][4 * s];
+        wsv[i] = ws[i][4 * s];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma_mx(wv[j], av[i], acc[i][j], wsv[j], asv[i]);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma_mx(wv[j], av[i], acc[i][j], wsv[j], asv[i]);
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = m0 + 16 * i + r, n = n0 + 16 * j + 4 * kg + e;
+          if (m < g.M && n < g.N) store_mx_one<OUT>(g, m, n, acc[i][j][e]);
+        }
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int m = m0 + 16 * i + r, n = n0 + 16 * j + 4 * kg + e;
-        if (m < g.M && n < g.N) store_mx_one<OUT>(g, m, n, acc[i][j][e]);
-      }
 }
 
 // ---------------------------------------------------------------------------
@@ -382,14 +384,22 @@ int launch_tile(const Mx4Gemm& g, hipStream_t stream) {
 
 }  // namespace
 
+// Times from problems of a quarter of a round to eight rounds at K = 1024 and 5120.
+static const MxTime kTimes[] = {
+    {1, 256, 256, 10000, 6100, 1790, 1900}, {5, 128, 256, 3500, 2700, 1070, 1117}, {6, 256, 128, 3500, 2700, 1070, 1117},
+    {2, 128, 128, 2700, 1000, 610, 579},    {3, 64, 128, 2700, 900, 430, 372},     {7, 128, 64, 2700, 1000, 412, 360},
+    {4, 64, 64, 2500, 1060, 319, 235},      {8, 32, 64, 2500, 850, 294, 174}};
+
+int choose_gemm_mxfp4(const Mx4Gemm& g) {
+  if (mx_rows_fit(false, g.M, g.N)) return kMxRows;
+  const int cus = cu_count();
+  return tiles_fit(g, 1) ? fastest_tile(kTimes, sizeof(kTimes) / sizeof(kTimes[0]), g, cus > 0 ? cus : 256) : 0;
+}
+
 int launch_gemm_mxfp4(const Mx4Gemm& g, int variant, hipStream_t stream) {
-  if (variant < 0 && mx_rows_fit(g.M)) return launch_gemm_mxfp4_rows(g, stream);
-  // (offsets inside a tile are 32 bits)
-  const bool small_strides = std::max({g.lda, g.ldas, g.ldb, g.ldbs, 4 * g.ldo}) * 256 < INT32_MAX;
-  if (variant < 0 && g.M > 32 && small_strides) {
-    const int64_t big = (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256), half = (int64_t)((g.M + 127) / 128) * ((g.N + 255) / 256);
-    variant = big >= 512 ? 1 : half >= 192 ? 5 : 2;
-  }
+  if (variant < 0) variant = choose_gemm_mxfp4(g);
+  if (variant == kMxRows && g.M <= 16) return launch_gemm_mxfp4_rows(g, stream);
+  if (!tiles_fit(g, 1)) variant = 0;
   switch (variant) {
     case 1: return launch_tile<MxTile<256, 256, 2, 2, 3, 2, 1>>(g, stream);
     case 2: return launch_tile<MxTile<128, 128, 2, 2, 3, 2, 2>>(g, stream);
@@ -397,8 +407,10 @@ int launch_gemm_mxfp4(const Mx4Gemm& g, int variant, hipStream_t stream) {
     case 4: return launch_tile<MxTile<64, 64, 2, 2, 4, 4, 2>>(g, stream);
     case 5: return launch_tile<MxTile<128, 256, 2, 2, 3, 3, 1>>(g, stream);
     case 6: return launch_tile<MxTile<256, 128, 2, 2, 3, 3, 1>>(g, stream);
+    case 7: return launch_tile<MxTile<128, 64, 2, 2, 3, 3, 2>>(g, stream);
+    case 8: return launch_tile<MxTile<32, 64, 1, 2, 4, 4, 3>>(g, stream);
   }
-  const dim3 grid((unsigned)((g.N + 127) / 128), (unsigned)((g.M + 31) / 32));
+  const dim3 grid((unsigned)((g.N + 127) / 128), (unsigned)std::min((g.M + 31) / 32, 65535));
   switch (g.out_dtype) {
     case CDIT_DT_F16: hipLaunchKernelGGL(gemm_mxfp4_direct<CDIT_DT_F16>, grid, dim3(256), 0, stream, g); break;
     case CDIT_DT_F32: hipLaunchKernelGGL(gemm_mxfp4_direct<CDIT_DT_F32>, grid, dim3(256), 0, stream, g); break;

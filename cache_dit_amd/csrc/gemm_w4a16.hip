@@ -19,55 +19,57 @@ __device__ __forceinline__ float mx_weight_scale(int e) { return e == kMxNan ? _
 // A wavefront per 32 x 32 outputs, operands straight from memory.
 __global__ __launch_bounds__(256) void gemm_w4a16_direct(Mx4Gemm g) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
-  const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 128 + wave * 32;
+  const int n0 = blockIdx.x * 128 + wave * 32;
   if (n0 >= g.N) return;
   const int blocks = g.K / kMxBlock, steps = (g.K + 127) / 128;
-  const uint8_t *a[2], *w[2], *ws[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t m = min(m0 + 16 * i + r, g.M - 1), n = min(n0 + 16 * i + r, g.N - 1);
-    a[i] = g.a + 2 * m * g.lda + 64 * kg;
-    w[i] = g.b + n * g.ldb + 16 * kg;
-    ws[i] = g.b_scale + n * g.ldbs + kg;
-  }
-  v4f acc[2][2] = {};
-  for (int s = 0; s < steps; ++s) {
-    const bool in = 4 * s + kg < blocks;  // behind K: zeros in both operands
-    v8bf av[2][4];
-    v4u wv[2];
-    float wsv[2];
+  for (int m0 = blockIdx.y * 32; m0 < g.M; m0 += gridDim.y * 32) {
+    const uint8_t *a[2], *w[2], *ws[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      const int64_t m = min(m0 + 16 * i + r, g.M - 1), n = min(n0 + 16 * i + r, g.N - 1);
+      a[i] = g.a + 2 * m * g.lda + 64 * kg;
+      w[i] = g.b + n * g.ldb + 16 * kg;
+      ws[i] = g.b_scale + n * g.ldbs + kg;
+    }
+    v4f acc[2][2] = {};
+    for (int s = 0; s < steps; ++s) {
+      const bool in = 4 * s + kg < blocks;  // behind K: zeros in both operands
+      v8bf av[2][4];
+      v4u wv[2];
+      float wsv[2];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const v4u z = {0, 0, 0, 0};
-        av[i][q] = __builtin_bit_cast(v8bf, in ? *reinterpret_cast<const v4u*>(a[i] + 256 * (int64_t)s + 16 * q) : z);
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const v4u z = {0, 0, 0, 0};
+          av[i][q] = __builtin_bit_cast(v8bf, in ? *reinterpret_cast<const v4u*>(a[i] + 256 * (int64_t)s + 16 * q) : z);
+        }
+        wv[i] = in ? *reinterpret_cast<const v4u*>(w[i] + 64 * (int64_t)s) : v4u{0, 0, 0, 0};
+        wsv[i] = in ? mx_weight_scale(ws[i][4 * s]) : 1.0f;
       }
-      wv[i] = in ? *reinterpret_cast<const v4u*>(w[i] + 64 * (int64_t)s) : v4u{0, 0, 0, 0};
-      wsv[i] = in ? mx_weight_scale(ws[i][4 * s]) : 1.0f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const v8bf b = mx_to_bf16(wv[j][q], wsv[j]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, av[i][q], acc[i][j], 0, 0, 0);
+        }
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const v8bf b = mx_to_bf16(wv[j][q], wsv[j]);
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, av[i][q], acc[i][j], 0, 0, 0);
-      }
+        for (int e = 0; e < 4; ++e) {
+          const int m = m0 + 16 * i + r, n = n0 + 16 * j + 4 * kg + e;
+          if (m >= g.M || n >= g.N) continue;
+          float v = acc[i][j][e];
+          if (g.bias) v += bias_to_f32<CDIT_DT_BF16>(static_cast<const uint16_t*>(g.bias)[n]);
+          if (g.epilogue & CDIT_EPI_GELU_TANH) v = gelu_tanh(v);
+          static_cast<uint16_t*>(g.out)[(int64_t)m * g.ldo + n] = (uint16_t)f32_to_bf16_bits(v);
+        }
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int m = m0 + 16 * i + r, n = n0 + 16 * j + 4 * kg + e;
-        if (m >= g.M || n >= g.N) continue;
-        float v = acc[i][j][e];
-        if (g.bias) v += bias_to_f32<CDIT_DT_BF16>(static_cast<const uint16_t*>(g.bias)[n]);
-        if (g.epilogue & CDIT_EPI_GELU_TANH) v = gelu_tanh(v);
-        static_cast<uint16_t*>(g.out)[(int64_t)m * g.ldo + n] = (uint16_t)f32_to_bf16_bits(v);
-      }
 }
 
 // ---------------------------------------------------------------------------
@@ -92,7 +94,7 @@ struct W4Tile {
   static constexpr int GROUP_M = BM >= 256 ? 4 : 8;
   static_assert(WM % 32 == 0 && WN % 32 == 0 && NDA >= 1 && NDB >= 1 && (TN == 1 || TN == 2 || TN == 4), "whole fragments, whole instructions");
   static_assert(WAVES % 2 == 0, "the chunk that a lane fetches is the same in each of its wavefront's instructions");
-  static_assert(SA >= 3 && SA <= 4 && FLY + NDB + 2 * TN <= 63 && LDS <= 160 * 1024, "a tile has four steps at least; vmcnt has 6 bits; LDS");
+  static_assert(SA >= 3 && SA <= 8 && FLY + NDB + 2 * TN <= 63 && LDS <= 160 * 1024, "a tile has eight steps at least; vmcnt has 6 bits; LDS");
 };
 
 template <class C>
@@ -301,12 +303,14 @@ gemm_w4a16_tile(Mx4Gemm g, int tiles_m, int tiles_n) {
         convert(s, 3);
         window(2 * MF + s);
       });
-      // (this step's scales and line instructions are younger than what has to have landed)
+      // (this step's scales and line instructions are younger than what has to have landed; behind a line's last, two
+      // windows go out before its codes are read)
       constexpr int YOUNG = T == 0 ? TN : 0, LINE = T == 0 ? (NDB + 1) / 2 : T == 1 ? NDB / 2 : 0;
+      constexpr int FLY = T == 3 && C::FLY > 2 * NDA ? 2 * NDA : C::FLY;
       if (b_due)
-        wait_and_barrier<C::FLY + YOUNG + LINE>();
+        wait_and_barrier<FLY + YOUNG + LINE>();
       else
-        wait_and_barrier<C::FLY + YOUNG>();
+        wait_and_barrier<FLY + YOUNG>();
       if (T == 3) order();
       quarter(std::integral_constant<int, 3>{}, [&](int s) {
         // codes first: they are converted in the second half
@@ -363,10 +367,151 @@ int launch_tile(const Mx4Gemm& g, hipStream_t stream) {
   return 0;
 }
 
+// ---------------------------------------------------------------------------
+// Few tiles (a prompt's rows): a workgroup per BM x BN outputs whose wavefronts split K as well. K advances in lines of 256; of
+// each, wavefront group g = 0 .. 3 takes the elements 64 g .. 64 g + 63 of the same 32 x 32 blocks, and the four partial sums
+// meet in LDS at the end. Such a problem has one workgroup a CU: with one wavefront per block, as in the tiles above, every
+// step of 64 waited for LDS reads and conversions that a single MFMA cannot cover (64 x 64 tiles, 77 x 5120 x 4096 (M x N x K):
+// 0.28 us a step of 64); four wavefronts per SIMD cover each other.
+template <int BM_, int BN_, int D_>
+struct W4Split {
+  static constexpr int BM = BM_, BN = BN_, D = D_, RB = BM / 32, CB = BN / 32, WAVES = 4 * RB * CB, THREADS = 64 * WAVES;
+  static constexpr int PANEL = BM * 128, A_BYTES = 4 * PANEL, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int JOIN = 3 * BM * BN * 4, LDS = D * STAGE > JOIN ? D * STAGE : JOIN;
+  static constexpr int NDMA = STAGE / 1024, ND = (NDMA + WAVES - 1) / WAVES;  // DMA instructions of a line, of a wavefront
+  static_assert(D >= 2 && (D - 1) * ND <= 63 && LDS <= 160 * 1024 && WAVES <= 16, "vmcnt has 6 bits; LDS");
+};
+
+template <class C>
+__global__ __launch_bounds__(C::THREADS) void gemm_w4a16_split(Mx4Gemm g, int tiles_m, int tiles_n) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  constexpr int D = C::D, ND = C::ND, WAVES = C::WAVES, STAGE = C::STAGE, PANEL = C::PANEL, A_BYTES = C::A_BYTES;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = wave / (C::RB * C::CB), blk = wave % (C::RB * C::CB), rb = blk / C::CB, cb = blk % C::CB;
+  const int r32 = lane & 31, h = lane >> 5;
+  int tm, tn;
+  tile_of_block<8>(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, &tm, &tn);
+  const int m0 = tm * C::BM, n0 = tn * C::BN;
+  const int KB = g.K / kMxBlock, KL = (g.K + 255) / 256, S = (g.K + 127) / 128 * 4;
+  const int rm = min(C::BM, g.M - m0) - 1, rn = min(C::BN, g.N - n0) - 1;
+  auto buffer = [](const uint8_t* p, int bytes) -> __amdgpu_buffer_rsrc_t {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, bytes, 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t a_buf = buffer(g.a + 2 * (int64_t)m0 * g.lda, 2 * (rm * (int)g.lda + g.K));
+  const __amdgpu_buffer_rsrc_t b_buf = buffer(g.b + (int64_t)n0 * g.ldb, rn * (int)g.ldb + g.K / 2);
+  const __amdgpu_buffer_rsrc_t s_buf = buffer(g.b_scale + (int64_t)n0 * g.ldbs, rn * (int)g.ldbs + S);
+
+  // DMA instruction q of a line fills 1 KiB: 8 rows of one of X's four panels, or of the codes; this wavefront's are wave +
+  // WAVES p.
+  auto dma = [&](int line, int stage) {
+#pragma unroll
+    for (int p = 0; p < ND; ++p) {
+      const int q = wave + WAVES * p;
+      if (q >= C::NDMA) continue;  // (uniform; the wait counts go by what this wavefront issues)
+      const int byte = q * 1024, panel = byte / PANEL, row = (byte % PANEL) / 128 + (lane >> 3);
+      const int chunk = (lane & 7) ^ ((row >> 1) & 7);
+      if (byte < A_BYTES) {
+        const int k = 256 * line + 64 * panel + 8 * chunk;
+        const int at = (int)(k < g.K ? (uint32_t)row * (uint32_t)g.lda * 2 + 2 * k : 0x80000000u);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(a_buf, (__attribute__((address_space(3))) void*)(smem + stage + byte), 16, at, 0, 0, 0);
+      } else {
+        const int brow = (byte - A_BYTES) / 128 + (lane >> 3), c = (lane & 7) ^ ((brow >> 1) & 7), block = 8 * line + c;
+        const int at = (int)(block < KB ? (uint32_t)brow * (uint32_t)g.ldb + 16 * block : 0x80000000u);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(b_buf, (__attribute__((address_space(3))) void*)(smem + stage + byte), 16, at, 0, 0, 0);
+      }
+    }
+  };
+  const int nd = C::NDMA / WAVES + (wave < C::NDMA % WAVES ? 1 : 0);  // instructions this wavefront issues for a line
+  auto wait_lines = [&](int later) {  // at most `later` lines of this wavefront's DMA in flight
+    if (nd == ND)
+      wait_steps<ND, D - 1, true>(later);
+    else
+      wait_steps<ND - 1, D - 1, true>(later);
+  };
+
+  // fragment maps: X's chunk 4 h + q of this group's panel; codes' chunk 2 grp + h
+  const int swz = (r32 >> 1) & 7;
+  const uint32_t rd_a = grp * PANEL + (32 * rb + r32) * 128, rd_b = A_BYTES + (32 * cb + r32) * 128 + (((2 * grp + h) ^ swz) << 4);
+  const uint32_t off_s = (uint32_t)(32 * cb + r32) * (uint32_t)g.ldbs + 4 * (grp >> 1);  // the word of this group's two bytes
+  auto load_scale = [&](int line) -> uint32_t {
+    const int at = (int)(8 * line + 4 * (grp >> 1) < S ? off_s + 8 * line : 0x80000000u);
+    return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(s_buf, at, 0, 0);
+  };
+  auto read = [&](const uint8_t* __restrict__ st, uint32_t at) -> v4u { return *reinterpret_cast<const v4u*>(st + at); };
+
+  v16f acc = {};
+  uint32_t sc = load_scale(0), sc_next = 0;
+#pragma unroll
+  for (int l = 0; l < D - 1; ++l)
+    if (l < KL) dma(l, l * STAGE);
+  int stage = 0, free_stage = (D - 1) * STAGE;
+  for (int l = 0; l < KL; ++l) {
+    wait_lines(min(D - 2, KL - 1 - l));  // line l has landed; everyone is done with line l - 1
+    if (l + 1 < KL) sc_next = load_scale(l + 1);
+    if (l + D - 1 < KL) dma(l + D - 1, free_stage);
+    const v4u c = read(smem + stage, rd_b);
+    v4u a[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) a[q] = read(smem + stage, rd_a + (((4 * h + q) ^ swz) << 4));
+    const int e = (sc >> (8 * (2 * (grp & 1) + h))) & 255;
+    const float f = e == kMxNan ? __uint_as_float(0x7fc00000u) : mx_scale_f32(e);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a[q]), mx_to_bf16(c[q], f), acc, 0, 0, 0);
+    sc = sc_next;
+    free_stage = stage;
+    stage = stage + STAGE == D * STAGE ? 0 : stage + STAGE;
+  }
+  // join: groups 1 .. 3 leave their sums, group 0 adds them in turn
+  wait_and_barrier<0>();
+  float* const join = reinterpret_cast<float*>(smem);
+  if (grp > 0) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) join[((grp - 1) * (C::RB * C::CB) + blk) * 1024 + 64 * e + lane] = acc[e];
+  }
+  __syncthreads();
+  if (grp > 0) return;
+  float bias[1];
+  mx_bias<1, CDIT_DT_BF16>(g, n0 + 32 * cb + r32, bias);
+  v16f out[1][1];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float v = acc[e];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) v += join[(k * (C::RB * C::CB) + blk) * 1024 + 64 * e + lane];
+    out[0][0][e] = v + bias[0];
+  }
+  store_mx_tile<1, 1, CDIT_DT_BF16>(out, g, m0, C::BM, 32 * rb + 4 * h, n0 + 32 * cb + r32);
+}
+
+template <class C>
+int launch_split(const Mx4Gemm& g, hipStream_t stream) {
+  static bool lds_allowed[64];
+  if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&gemm_w4a16_split<C>), C::LDS, lds_allowed)) return rc;
+  const int tiles_m = (g.M + C::BM - 1) / C::BM, tiles_n = (g.N + C::BN - 1) / C::BN;
+  hipLaunchKernelGGL(gemm_w4a16_split<C>, dim3((unsigned)(tiles_m * tiles_n)), dim3(C::THREADS), C::LDS, stream, g, tiles_m,
+                     tiles_n);
+  return 0;
+}
+
 }  // namespace
 
+// Times from problems of a quarter of a round to eight rounds at K = 1024 and 5120.
+static const MxTime kTimes[] = {
+    {1, 256, 256, 3500, 15800, 5775, 5300}, {5, 128, 256, 2700, 2750, 3575, 3190}, {6, 256, 128, 2700, 3000, 3510, 3040},
+    {2, 128, 128, 2700, 900, 1940, 1750},   {3, 64, 128, 2700, 700, 1380, 1090},   {7, 128, 64, 2700, 700, 1220, 1150},
+    {4, 64, 64, 2300, 900, 1000, 681},      {8, 32, 64, 1800, 1200, 780, 836}};
+
+int choose_gemm_w4a16(const Mx4Gemm& g) {
+  if (mx_rows_fit(true, g.M, g.N)) return kMxRows;
+  const int cus = cu_count();
+  return tiles_fit(g, 2) ? fastest_tile(kTimes, sizeof(kTimes) / sizeof(kTimes[0]), g, cus > 0 ? cus : 256) : 0;
+}
+
 int launch_gemm_w4a16(const Mx4Gemm& g, int variant, hipStream_t stream) {
-  if (variant < 0 && mx_rows_fit(g.M)) return launch_gemm_w4a16_rows(g, stream);
+  if (variant < 0) variant = choose_gemm_w4a16(g);
+  if (variant == kMxRows && g.M <= 16) return launch_gemm_w4a16_rows(g, stream);
+  if (!tiles_fit(g, 2)) variant = 0;
   switch (variant) {
     case 1: return launch_tile<W4Tile<256, 256, 2, 2, 3, 1>>(g, stream);
     case 2: return launch_tile<W4Tile<128, 128, 2, 2, 3, 2>>(g, stream);
@@ -374,8 +519,10 @@ int launch_gemm_w4a16(const Mx4Gemm& g, int variant, hipStream_t stream) {
     case 4: return launch_tile<W4Tile<64, 64, 2, 2, 4, 2>>(g, stream);
     case 5: return launch_tile<W4Tile<128, 256, 2, 2, 4, 1>>(g, stream);
     case 6: return launch_tile<W4Tile<256, 128, 2, 2, 4, 1>>(g, stream);
+    case 7: return launch_tile<W4Tile<128, 64, 2, 2, 4, 2>>(g, stream);
+    case 8: return launch_split<W4Split<32, 64, 4>>(g, stream);
   }
-  const dim3 grid((unsigned)((g.N + 127) / 128), (unsigned)((g.M + 31) / 32));
+  const dim3 grid((unsigned)((g.N + 127) / 128), (unsigned)std::min((g.M + 31) / 32, 65535));
   hipLaunchKernelGGL(gemm_w4a16_direct, grid, dim3(256), 0, stream, g);
   return 0;
 }

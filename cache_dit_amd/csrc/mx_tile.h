@@ -4,12 +4,41 @@
 #ifndef CDIT_MX_TILE_H_
 #define CDIT_MX_TILE_H_
 
+#include <algorithm>
 #include <type_traits>
 
 #include "gemm_common.h"
 
 namespace cdit {
 namespace {
+
+// A tile and its measured times, ns: of a launch, and per tile on the fullest CU; of a step of 256 along K, for a CU's only
+// tile and for each of several (which run on the CU together, or one after the other).
+struct MxTime {
+  int variant, bm, bn, start, tile, lone, step;
+};
+// The tile with the least time. Tiles beyond whole rounds of the CUs count half a round and half their share of one: fewer CUs
+// share the memory and the power then.
+inline int fastest_tile(const MxTime* t, int count, const Mx4Gemm& g, int cus) {
+  const int64_t steps = (g.K + 255) / 256;
+  int best = -1;
+  int64_t best_ns = 0;
+  for (int i = 0; i < count; ++i) {
+    const int64_t tiles = (int64_t)((g.M + t[i].bm - 1) / t[i].bm) * ((g.N + t[i].bn - 1) / t[i].bn);
+    const int64_t permille = tiles <= cus ? 1000 : rounds_permille(tiles, cus, 500, 500);
+    const int64_t ns = t[i].start + t[i].tile * permille / 1000 + steps * std::max<int64_t>(t[i].lone, t[i].step * permille / 1000);
+    if (best < 0 || ns < best_ns) {
+      best = t[i].variant;
+      best_ns = ns;
+    }
+  }
+  return best;
+}
+// Offsets inside a tile are 32 bits; tiles are counted in 32 bits.
+inline bool tiles_fit(const Mx4Gemm& g, int a_bytes) {
+  const int64_t widest = std::max({g.lda * a_bytes, g.ldas, g.ldb, g.ldbs, 4 * g.ldo, (int64_t)g.K * 2});
+  return widest * 256 < INT32_MAX && ((int64_t)g.M / 32 + 1) * ((int64_t)g.N / 64 + 1) < INT32_MAX;
+}
 
 // The bias of a lane's columns in fp32; 0 for columns that do not exist, and without a bias.
 template <int TN, int OUT>
