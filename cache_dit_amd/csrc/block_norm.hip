@@ -108,8 +108,23 @@ struct BlockSum {
   }
 };
 
+// The codes of a piece c of y as it is (or would be) stored. K is a multiple of 32: the quad of lanes that holds a block is in the
+// row, and here, as a whole.
+template <int DT>
+__device__ __forceinline__ void put_codes(const Args& a, int64_t row, int c, const Mx8<DT>& v) {
+  const int e = mx_exponent(mx_quad_max(mx_amax8<DT>(v)));
+  *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.codes) + row * a.ld_codes + 4 * c) = mx_codes8<DT>(v, e);
+  if (c % 4 == 0) {
+    uint8_t* const s = static_cast<uint8_t*>(a.code_scales) + row * a.ld_code_scales;
+    const int b = c / 4, blocks = (int)a.K / kMxBlock;
+    s[b] = (uint8_t)e;
+    if (b == blocks - 1)
+      for (int pad = blocks; pad % 4 != 0; ++pad) s[pad] = (uint8_t)kMxPad;
+  }
+}
+
 // A piece of 8 columns of the row: where it is, and what of it exists.
-template <int ST, int DT, bool VEC>
+template <int ST, int DT>
 struct Row {
   const Args& a;
   int64_t row;
@@ -117,12 +132,12 @@ struct Row {
   __device__ __forceinline__ void vec(const void* p, int64_t ld, int64_t rows_per, int c, float (&f)[8]) const {
     const int64_t at = (rows_per > 0 ? row / rows_per * ld : 0) + 8 * c;
     if (a.vec_f32)
-      load8<CDIT_DT_F32, VEC>(static_cast<const float*>(p) + at, n_of(c), f);
+      load8<CDIT_DT_F32, false>(static_cast<const float*>(p) + at, n_of(c), f);
     else
-      load8<DT, VEC>(static_cast<const uint8_t*>(p) + at * size_of<DT>(), n_of(c), f);
+      load8<DT, false>(static_cast<const uint8_t*>(p) + at * size_of<DT>(), n_of(c), f);
   }
   __device__ __forceinline__ void branch(int c, float (&t)[8]) const {
-    load8<DT, VEC>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + 8 * c) * size_of<DT>(), n_of(c), t);
+    load8<DT, false>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + 8 * c) * size_of<DT>(), n_of(c), t);
   }
   // t -> post norm of t; mean and rstd of the branch's row
   __device__ __forceinline__ void post(int c, float mean, float rstd, float (&t)[8]) const {
@@ -132,7 +147,7 @@ struct Row {
     for (int i = 0; i < 8; ++i) t[i] = (t[i] - mean) * rstd * (a.post_weight ? w[i] : 1.0f);
   }
   __device__ __forceinline__ void stream(int c, float (&x)[8]) const {
-    load8<ST, VEC>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + 8 * c) * size_of<ST>(), n_of(c), x);
+    load8<ST, false>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + 8 * c) * size_of<ST>(), n_of(c), x);
   }
   // t, x -> h
   __device__ __forceinline__ void residual(int c, const float (&x)[8], float (&t)[8]) const {
@@ -162,23 +177,11 @@ struct Row {
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += f[i];
     }
-    store8<ST, VEC>(static_cast<uint8_t*>(a.h) + (row * a.ld_h + 8 * c) * size_of<ST>(), n, h);
-    if (a.y) store8<DT, VEC>(static_cast<uint8_t*>(a.y) + (row * a.ld_y + 8 * c) * size_of<DT>(), n, y);
+    store8<ST, false>(static_cast<uint8_t*>(a.h) + (row * a.ld_h + 8 * c) * size_of<ST>(), n, h);
+    if (a.y) store8<DT, false>(static_cast<uint8_t*>(a.y) + (row * a.ld_y + 8 * c) * size_of<DT>(), n, y);
     if (a.codes) {
-      // the codes of y as it is (or would be) stored; K is a multiple of 32, so that the quad of lanes
-      // that holds a block is in the row as a whole
       const Mx8<DT> v = narrow8<DT>(y);
-      const int e = mx_exponent(mx_quad_max(mx_amax8<DT>(v)));
-      if (n > 0) {
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.codes) + row * a.ld_codes + 4 * c) = mx_codes8<DT>(v, e);
-        uint8_t* const s = static_cast<uint8_t*>(a.code_scales) + row * a.ld_code_scales;
-        if (c % 4 == 0) {
-          const int b = c / 4, blocks = (int)a.K / kMxBlock;
-          s[b] = (uint8_t)e;
-          if (b == blocks - 1)
-            for (int pad = blocks; pad % 4 != 0; ++pad) s[pad] = (uint8_t)kMxPad;
-        }
-      }
+      if (n > 0) put_codes<DT>(a, row, c, v);
     }
   }
 };
@@ -223,7 +226,7 @@ __global__ __launch_bounds__(256) void gate_residual_norm_any(Args a) {
   const int pieces = (int)((a.K + 7) / 8);
   // (whole quads of lanes take part in a block's maximum, also behind the last piece)
   for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-    const Row<ST, DT, false> r{a, row};
+    const Row<ST, DT> r{a, row};
     float pm = 0.0f, pr = 1.0f, mean, rstd;
     if (a.post_norm)
       statistics(a, a.post_norm == CDIT_NORM_LAYER, sum, threadIdx.x, 256, pieces,
@@ -245,32 +248,79 @@ __global__ __launch_bounds__(256) void gate_residual_norm_any(Args a) {
 }
 
 // The row in registers: CH pieces per lane, WAVES wavefronts per row, 16-byte accesses. A workgroup takes a run of consecutive
-// rows; the next row's loads are under way while a row is worked on.
+// rows; the next row's loads are under way while a row is worked on, and the vectors, folded into one factor of the branch and a
+// factor and an addend of the result, stay in registers until a row takes others.
 template <int ST, int DT, int WAVES, int CH>
 __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, int rows_per_wg) {
   __shared__ float slots[2][WAVES];
   BlockSum<WAVES> sum{slots, 0};
   const int64_t row0 = (int64_t)blockIdx.x * rows_per_wg, row_end = min(a.M, row0 + rows_per_wg);
+  if (row0 >= row_end) return;
   const float inv_k = 1.0f / (float)a.K;
-  Mx8<DT> b_raw[2][CH];
-  Mx8<ST> x_raw[2][CH];
-  auto piece = [&](int c) { return (c * WAVES + (int)(threadIdx.x >> 6)) * 64 + (int)(threadIdx.x & 63); };
+  const bool post_layer = a.post_norm == CDIT_NORM_LAYER, layer = a.norm == CDIT_NORM_LAYER;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int col[CH];  // first column of a piece
+  bool in[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    col[c] = 8 * ((c * WAVES + wave) * 64 + lane);
+    in[c] = col[c] < a.K;
+  }
   auto fetch = [&](int64_t row, Mx8<DT>(&bb)[CH], Mx8<ST>(&xx)[CH]) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       bb[c] = {};
       xx[c] = {};
-      if (8 * piece(c) < a.K) {
-        bb[c] = mx_load8<DT>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + 8 * piece(c)) * size_of<DT>());
-        xx[c] = mx_load8<ST>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + 8 * piece(c)) * size_of<ST>());
+      if (in[c]) {
+        bb[c] = mx_load8<DT>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + col[c]) * size_of<DT>());
+        xx[c] = mx_load8<ST>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + col[c]) * size_of<ST>());
+      }
+    }
+  };
+  // gate * post_weight; norm_weight * (1 + scale); shift
+  float vg[CH][8], vm[CH][8], vs[CH][8];
+  int64_t at_gate = -1, at_shift = -1, at_scale = -1;
+  auto vector = [&](const void* p, int64_t at, int c, float(&f)[8]) {
+    if (a.vec_f32)
+      load8<CDIT_DT_F32, true>(static_cast<const float*>(p) + at + col[c], in[c] ? 8 : 0, f);
+    else
+      load8<DT, true>(static_cast<const uint8_t*>(p) + (at + col[c]) * size_of<DT>(), in[c] ? 8 : 0, f);
+  };
+  auto take_vectors = [&](int64_t row) {
+    const int64_t ig = a.gate ? row / a.rows_per_gate : 0, ih = a.shift ? row / a.rows_per_shift : 0,
+                  ic = a.scale ? row / a.rows_per_scale : 0;
+    if (ig == at_gate && ih == at_shift && ic == at_scale) return;  // uniform
+    at_gate = ig;
+    at_shift = ih;
+    at_scale = ic;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        vg[c][i] = vm[c][i] = 1.0f;
+        vs[c][i] = 0.0f;
+      }
+      if (a.gate) vector(a.gate, ig * a.ld_gate, c, vg[c]);
+      if (a.shift) vector(a.shift, ih * a.ld_shift, c, vs[c]);
+      if (a.norm_weight) vector(a.norm_weight, 0, c, vm[c]);
+      if (a.post_weight) {
+        vector(a.post_weight, 0, c, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vg[c][i] *= f[i];
+      }
+      if (a.scale) {
+        vector(a.scale, ic * a.ld_scale, c, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vm[c][i] = __fmaf_rn(vm[c][i], f[i], vm[c][i]);
       }
     }
   };
   // mean and 1 / sqrt(...) of the row whose pieces are f, as in statistics()
-  auto stats = [&](const float(&f)[CH][8], bool layer, float* mean, float* rstd) {
+  auto stats = [&](const float(&f)[CH][8], bool centred, float* mean, float* rstd) {
     float s = 0.0f;
     *mean = 0.0f;
-    if (layer) {
+    if (centred) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -279,40 +329,46 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
       s = 0.0f;
     }
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const bool in = 8 * piece(c) < a.K;
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float d = in ? f[c][i] - *mean : 0.0f;
+        const float d = in[c] ? f[c][i] - *mean : 0.0f;
         s = __fmaf_rn(d, d, s);
       }
-    }
     *rstd = 1.0f / __fsqrt_rn(sum(s) * inv_k + a.eps);
   };
   auto one_row = [&](int64_t row, Mx8<DT>(&bb)[CH], Mx8<ST>(&xx)[CH], Mx8<DT>(&nb)[CH], Mx8<ST>(&nx)[CH]) {
     if (row + 1 < row_end) fetch(row + 1, nb, nx);
-    const Row<ST, DT, true> r{a, row};
-    float h[CH][8], mean, rstd;
+    take_vectors(row);
+    float h[CH][8], mean = 0.0f, rstd = 1.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) widen8<DT>(bb[c], h[c]);
-    if (a.post_norm) {
-      stats(h, a.post_norm == CDIT_NORM_LAYER, &mean, &rstd);
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-        if (8 * piece(c) < a.K) r.post(piece(c), mean, rstd, h[c]);
-    }
+    if (a.post_norm) stats(h, post_layer, &mean, &rstd);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       float x[8];
       widen8<ST>(xx[c], x);
-      if (8 * piece(c) < a.K) r.residual(piece(c), x, h[c]);
-    }
-    stats(h, a.norm == CDIT_NORM_LAYER, &mean, &rstd);
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-      if (8 * piece(c) < a.K) r.finish(piece(c), mean, rstd, h[c]);
+      for (int i = 0; i < 8; ++i) {
+        const float t = (h[c][i] - mean) * rstd;
+        h[c][i] = in[c] ? __fmaf_rn(vg[c][i], t, a.residual_scale * x[i]) : 0.0f;
+      }
+    }
+    stats(h, layer, &mean, &rstd);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if (!in[c]) continue;
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __fmaf_rn((h[c][i] - mean) * rstd, vm[c][i], vs[c][i]);
+      mx_store8<ST>(static_cast<uint8_t*>(a.h) + (row * a.ld_h + col[c]) * size_of<ST>(), narrow8<ST>(h[c]));
+      const Mx8<DT> v = narrow8<DT>(y);
+      if (a.y) mx_store8<DT>(static_cast<uint8_t*>(a.y) + (row * a.ld_y + col[c]) * size_of<DT>(), v);
+      if (a.codes) put_codes<DT>(a, row, col[c] / 8, v);
+    }
   };
-  if (row0 >= row_end) return;
+  Mx8<DT> b_raw[2][CH];
+  Mx8<ST> x_raw[2][CH];
   fetch(row0, b_raw[0], x_raw[0]);
   for (int64_t row = row0; row < row_end; row += 2) {
     one_row(row, b_raw[0], x_raw[0], b_raw[1], x_raw[1]);
@@ -351,13 +407,15 @@ int launch_types(const Args& a, hipStream_t stream) {
     return 0;                                                                                                         \
   }
     CDIT_NORM_CASE(1, 1)
-    CDIT_NORM_CASE(1, 2)
-    CDIT_NORM_CASE(2, 2)
-    CDIT_NORM_CASE(3, 2)
-    CDIT_NORM_CASE(4, 2)
-    CDIT_NORM_CASE(5, 2)
-    CDIT_NORM_CASE(6, 2)
-    CDIT_NORM_CASE(8, 2)
+    CDIT_NORM_CASE(2, 1)
+    CDIT_NORM_CASE(3, 1)
+    CDIT_NORM_CASE(4, 1)
+    CDIT_NORM_CASE(5, 1)
+    CDIT_NORM_CASE(6, 1)
+    CDIT_NORM_CASE(8, 1)
+    CDIT_NORM_CASE(10, 1)
+    CDIT_NORM_CASE(12, 1)
+    CDIT_NORM_CASE(16, 1)
     CDIT_NORM_CASE(12, 2)
     CDIT_NORM_CASE(16, 2)
 #undef CDIT_NORM_CASE

@@ -400,8 +400,12 @@ int launch_gemm_mxfp4(const Mx4Gemm& g, int variant, hipStream_t stream) {
   if (variant < 0) variant = choose_gemm_mxfp4(g);
   if (variant == kMxRows && g.M <= 16) return launch_gemm_mxfp4_rows(g, stream);
   if (!tiles_fit(g, 1)) variant = 0;
+  if (variant == 1 && g.out_dtype == CDIT_DT_F32) variant = 5;  // (no registers left for 16-byte stores of 256 x 256)
   switch (variant) {
-    case 1: return launch_tile<MxTile<256, 256, 2, 2, 3, 2, 1>>(g, stream);
+    case 1: {
+      using C = MxTile<256, 256, 2, 2, 3, 2, 1>;
+      return g.out_dtype == CDIT_DT_F16 ? launch_tile_out<C, CDIT_DT_F16>(g, stream) : launch_tile_out<C, CDIT_DT_BF16>(g, stream);
+    }
     case 2: return launch_tile<MxTile<128, 128, 2, 2, 3, 2, 2>>(g, stream);
     case 3: return launch_tile<MxTile<64, 128, 2, 2, 3, 3, 2>>(g, stream);
     case 4: return launch_tile<MxTile<64, 64, 2, 2, 4, 4, 2>>(g, stream);

@@ -3,6 +3,8 @@
 // A lane takes 8 consecutive elements (16 bytes of a 16-bit type), so that a wavefront reads 1 KiB in a
 // row; the four lanes of a quad hold the 32 elements of a block, whose largest magnitude meets in two DPP
 // steps; the hardware converters do scaling and rounding. Nothing goes through LDS.
+#include <algorithm>
+
 #include "cdit_internal.h"
 #include "mxfp4_device.h"
 
@@ -11,17 +13,23 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Which rows a workgroup takes, so that short rows share one: a run of `rows`, walked as one line of
-// `rows * per_row` pieces of 8 elements. Piece -> row by a multiplication: magic = ceil(2^32 / per_row) is
-// exact while piece * per_row < 2^32 (at most 2^12 pieces where rows > 1, checked by the launcher).
+// Which pieces of 8 elements a workgroup takes: `span` of a run of `rows` rows, walked as one line of rows * per_row pieces, so that
+// short rows share a workgroup and long ones are shared. Piece -> row by a multiplication: magic = ceil(2^32 / per_row) is exact
+// while piece * per_row < 2^32 (at most 2^11 pieces where rows > 1).
 struct Runs {
-  int rows, per_row;
+  int rows, per_row, span;
   uint32_t magic;
+  dim3 grid(int64_t M) const {
+    return dim3((unsigned)((M + rows - 1) / rows), (unsigned)((rows * per_row + span - 1) / span));
+  }
 };
-Runs runs_of(int64_t K) {
+// 2048 pieces a workgroup, eight a thread, where there are many; one a thread where that leaves CUs idle.
+Runs runs_of(int64_t M, int64_t K) {
   const int per_row = (int)(K / 8);
   const int rows = per_row >= 1024 ? 1 : 2048 / per_row;
-  return {rows, per_row, per_row == 1 ? 0u : (uint32_t)(((uint64_t(1) << 32) + per_row - 1) / per_row)};
+  const int64_t pieces = M * per_row, wanted = 4 * 256;
+  const int span = (int)std::min<int64_t>(2048, std::max<int64_t>(kThreads, (pieces / wanted + kThreads - 1) / kThreads * kThreads));
+  return {rows, per_row, span, (uint32_t)(((uint64_t(1) << 32) + per_row - 1) / per_row)};
 }
 __device__ __forceinline__ void locate(const Runs& r, uint32_t piece, uint32_t* row, uint32_t* at) {
   *row = r.rows == 1 ? 0u : __umulhi(piece, r.magic);
@@ -35,9 +43,10 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quant_rows(const uint8_t* __re
                                                              int64_t M, Runs r) {
   constexpr int ES = DT == CDIT_DT_F32 ? 4 : 2;
   const int64_t row0 = (int64_t)blockIdx.x * r.rows;
-  const uint32_t n = (uint32_t)min((int64_t)r.rows, M - row0) * (uint32_t)r.per_row;
+  const uint32_t n = (uint32_t)min((int64_t)r.rows, M - row0) * (uint32_t)r.per_row, first = blockIdx.y * (uint32_t)r.span;
+  const uint32_t end = min(n, first + (uint32_t)r.span);
   const int blocks = r.per_row / 4;
-  for (uint32_t p = threadIdx.x; p < n; p += kThreads) {
+  for (uint32_t p = first + threadIdx.x; p < end; p += kThreads) {
     uint32_t dr, at;
     locate(r, p, &dr, &at);
     const int64_t row = row0 + dr;
@@ -62,8 +71,9 @@ __global__ __launch_bounds__(kThreads) void mxfp4_dequant_rows(const uint8_t* __
                                                                Runs r) {
   constexpr int ES = DT == CDIT_DT_F32 ? 4 : 2;
   const int64_t row0 = (int64_t)blockIdx.x * r.rows;
-  const uint32_t n = (uint32_t)min((int64_t)r.rows, M - row0) * (uint32_t)r.per_row;
-  for (uint32_t p = threadIdx.x; p < n; p += kThreads) {
+  const uint32_t n = (uint32_t)min((int64_t)r.rows, M - row0) * (uint32_t)r.per_row, first = blockIdx.y * (uint32_t)r.span;
+  const uint32_t end = min(n, first + (uint32_t)r.span);
+  for (uint32_t p = first + threadIdx.x; p < end; p += kThreads) {
     uint32_t dr, at;
     locate(r, p, &dr, &at);
     const int64_t row = row0 + dr;
@@ -77,8 +87,8 @@ __global__ __launch_bounds__(kThreads) void mxfp4_dequant_rows(const uint8_t* __
 
 int launch_mxfp4_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ld_x, void* codes, int64_t ld_codes,
                        void* scales, int64_t ld_scales, hipStream_t stream) {
-  const Runs r = runs_of(K);
-  const dim3 grid((unsigned)((M + r.rows - 1) / r.rows));
+  const Runs r = runs_of(M, K);
+  const dim3 grid = r.grid(M);
 #define CDIT_MXQ(DT)                                                                                        \
   hipLaunchKernelGGL(mxfp4_quant_rows<DT>, grid, dim3(kThreads), 0, stream, static_cast<const uint8_t*>(x), \
                      ld_x, static_cast<uint8_t*>(codes), ld_codes, static_cast<uint8_t*>(scales), ld_scales, M, r)
@@ -94,8 +104,8 @@ int launch_mxfp4_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t l
 
 int launch_mxfp4_dequant(const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int64_t M, int64_t K,
                          void* out, int dtype, int64_t ld_out, hipStream_t stream) {
-  const Runs r = runs_of(K);
-  const dim3 grid((unsigned)((M + r.rows - 1) / r.rows));
+  const Runs r = runs_of(M, K);
+  const dim3 grid = r.grid(M);
 #define CDIT_MXD(DT)                                                                                             \
   hipLaunchKernelGGL(mxfp4_dequant_rows<DT>, grid, dim3(kThreads), 0, stream, static_cast<const uint8_t*>(codes), \
                      ld_codes, static_cast<const uint8_t*>(scales), ld_scales, static_cast<uint8_t*>(out), ld_out, M, r)
