@@ -249,8 +249,14 @@ __global__ __launch_bounds__(256) void gate_residual_norm_any(Args a) {
 
 // The row in registers: CH pieces per lane, WAVES wavefronts per row, 16-byte accesses. A workgroup takes a run of consecutive
 // rows; the next row's loads are under way while a row is worked on, and the vectors, folded into one factor of the branch and a
-// factor and an addend of the result, stay in registers until a row takes others.
-template <int ST, int DT, int WAVES, int CH>
+// factor and an addend of the result, stay in registers until a row takes others (with one piece a lane; with two, where the
+// registers of 16 wavefronts would not hold them, each row reads them again from the caches). us, 32760 x 5120, fp32 stream,
+// one set of vectors: 604 with the vectors read for each row, 417 so (4.8 TB/s; a copy of 1 GiB runs at 5.1).
+// ONCE: the 16-bit ones of x, branch and h are read and written non-temporally: they leave the caches to y or its codes, which the
+// next kernel reads. bf16, us, without and with: 8192 x 4096 with vectors per token 109 and 85 (5.5 TB/s), 4096 x 15360 126 and 114,
+// 32760 x 5120 291 and 290; below kOnceBytes, where the caches hold all of it, 2 x 4096 x 2560 36 and 42.
+constexpr int64_t kOnceBytes = (int64_t)64 << 20;
+template <int ST, int DT, int WAVES, int CH, bool ONCE>
 __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, int rows_per_wg) {
   __shared__ float slots[2][WAVES];
   BlockSum<WAVES> sum{slots, 0};
@@ -272,19 +278,48 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
       bb[c] = {};
       xx[c] = {};
       if (in[c]) {
-        bb[c] = mx_load8<DT>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + col[c]) * size_of<DT>());
-        xx[c] = mx_load8<ST>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + col[c]) * size_of<ST>());
+        bb[c] = mx_load8<DT, (ONCE && DT != CDIT_DT_F32)>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + col[c]) * size_of<DT>());
+        xx[c] = mx_load8<ST, (ONCE && ST != CDIT_DT_F32)>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + col[c]) * size_of<ST>());
       }
     }
   };
   // gate * post_weight; norm_weight * (1 + scale); shift
-  float vg[CH][8], vm[CH][8], vs[CH][8];
+  constexpr bool KEEP = CH == 1;
+  constexpr int KEPT = KEEP ? CH : 1;
+  float vg[KEPT][8], vm[KEPT][8], vs[KEPT][8];
   int64_t at_gate = -1, at_shift = -1, at_scale = -1;
   auto vector = [&](const void* p, int64_t at, int c, float(&f)[8]) {
     if (a.vec_f32)
       load8<CDIT_DT_F32, true>(static_cast<const float*>(p) + at + col[c], in[c] ? 8 : 0, f);
     else
       load8<DT, true>(static_cast<const uint8_t*>(p) + (at + col[c]) * size_of<DT>(), in[c] ? 8 : 0, f);
+  };
+  auto branch_factor = [&](int c, float(&f)[8]) {
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 1.0f;
+    if (a.gate) vector(a.gate, at_gate * a.ld_gate, c, f);
+    if (a.post_weight) {
+      vector(a.post_weight, 0, c, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] *= w[i];
+    }
+  };
+  auto result_factor = [&](int c, float(&f)[8]) {
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 1.0f;
+    if (a.norm_weight) vector(a.norm_weight, 0, c, f);
+    if (a.scale) {
+      vector(a.scale, at_scale * a.ld_scale, c, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = __fmaf_rn(f[i], w[i], f[i]);
+    }
+  };
+  auto result_addend = [&](int c, float(&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 0.0f;
+    if (a.shift) vector(a.shift, at_shift * a.ld_shift, c, f);
   };
   auto take_vectors = [&](int64_t row) {
     const int64_t ig = a.gate ? row / a.rows_per_gate : 0, ih = a.shift ? row / a.rows_per_shift : 0,
@@ -293,26 +328,12 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
     at_gate = ig;
     at_shift = ih;
     at_scale = ic;
+    if constexpr (KEEP) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        vg[c][i] = vm[c][i] = 1.0f;
-        vs[c][i] = 0.0f;
-      }
-      if (a.gate) vector(a.gate, ig * a.ld_gate, c, vg[c]);
-      if (a.shift) vector(a.shift, ih * a.ld_shift, c, vs[c]);
-      if (a.norm_weight) vector(a.norm_weight, 0, c, vm[c]);
-      if (a.post_weight) {
-        vector(a.post_weight, 0, c, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vg[c][i] *= f[i];
-      }
-      if (a.scale) {
-        vector(a.scale, ic * a.ld_scale, c, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vm[c][i] = __fmaf_rn(vm[c][i], f[i], vm[c][i]);
+      for (int c = 0; c < CH; ++c) {
+        branch_factor(c, vg[c]);
+        result_factor(c, vm[c]);
+        result_addend(c, vs[c]);
       }
     }
   };
@@ -346,22 +367,29 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
     if (a.post_norm) stats(h, post_layer, &mean, &rstd);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      float x[8];
+      float x[8], f[8];
       widen8<ST>(xx[c], x);
+      if constexpr (!KEEP) branch_factor(c, f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float t = (h[c][i] - mean) * rstd;
-        h[c][i] = in[c] ? __fmaf_rn(vg[c][i], t, a.residual_scale * x[i]) : 0.0f;
+        h[c][i] = in[c] ? __fmaf_rn(KEEP ? vg[KEEP ? c : 0][i] : f[i], t, a.residual_scale * x[i]) : 0.0f;
       }
     }
     stats(h, layer, &mean, &rstd);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       if (!in[c]) continue;
-      float y[8];
+      float y[8], m[8], s[8];
+      if constexpr (!KEEP) {
+        result_factor(c, m);
+        result_addend(c, s);
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __fmaf_rn((h[c][i] - mean) * rstd, vm[c][i], vs[c][i]);
-      mx_store8<ST>(static_cast<uint8_t*>(a.h) + (row * a.ld_h + col[c]) * size_of<ST>(), narrow8<ST>(h[c]));
+      for (int i = 0; i < 8; ++i)
+        y[i] = __fmaf_rn((h[c][i] - mean) * rstd, KEEP ? vm[KEEP ? c : 0][i] : m[i], KEEP ? vs[KEEP ? c : 0][i] : s[i]);
+      mx_store8<ST, (ONCE && ST != CDIT_DT_F32)>(static_cast<uint8_t*>(a.h) + (row * a.ld_h + col[c]) * size_of<ST>(),
+                                                 narrow8<ST>(h[c]));
       const Mx8<DT> v = narrow8<DT>(y);
       if (a.y) mx_store8<DT>(static_cast<uint8_t*>(a.y) + (row * a.ld_y + col[c]) * size_of<DT>(), v);
       if (a.codes) put_codes<DT>(a, row, col[c] / 8, v);
@@ -398,12 +426,16 @@ int launch_types(const Args& a, hipStream_t stream) {
       return CDIT_EHIP;
     }
     const int pieces = (int)(a.K / 8);
+    const bool once = 2 * a.M * a.K >= kOnceBytes;
 #define CDIT_NORM_CASE(W, CH)                                                                                         \
   if (pieces <= 64 * W * CH) {                                                                                        \
     const int64_t target = (int64_t)cus * std::max(1, 24 / W);                                                        \
     const int per = (int)std::min<int64_t>((a.M + target - 1) / target, 1 << 20);                                     \
-    hipLaunchKernelGGL((gate_residual_norm_rows<ST, DT, W, CH>), dim3((unsigned)((a.M + per - 1) / per)), dim3(64 * W), 0, \
-                       stream, a, per);                                                                               \
+    const dim3 grid((unsigned)((a.M + per - 1) / per));                                                               \
+    if (once)                                                                                                         \
+      hipLaunchKernelGGL((gate_residual_norm_rows<ST, DT, W, CH, DT != CDIT_DT_F32>), grid, dim3(64 * W), 0, stream, a, per); \
+    else                                                                                                              \
+      hipLaunchKernelGGL((gate_residual_norm_rows<ST, DT, W, CH, false>), grid, dim3(64 * W), 0, stream, a, per);     \
     return 0;                                                                                                         \
   }
     CDIT_NORM_CASE(1, 1)

@@ -43,14 +43,15 @@ template <int DT>
 struct Mx8 {
   uint32_t w[DT == CDIT_DT_F32 ? 8 : 4];
 };
-template <int DT>
+template <int DT, bool ONCE = false>  // ONCE: non-temporal, read by nobody else soon
 __device__ __forceinline__ Mx8<DT> mx_load8(const void* p) {
   Mx8<DT> v;
-  const mx_v4u a = *reinterpret_cast<const mx_v4u*>(p);
+  auto load = [](const mx_v4u* q) { return ONCE ? __builtin_nontemporal_load(q) : *q; };
+  const mx_v4u a = load(reinterpret_cast<const mx_v4u*>(p));
 #pragma unroll
   for (int i = 0; i < 4; ++i) v.w[i] = a[i];
   if constexpr (DT == CDIT_DT_F32) {
-    const mx_v4u b = *(reinterpret_cast<const mx_v4u*>(p) + 1);
+    const mx_v4u b = load(reinterpret_cast<const mx_v4u*>(p) + 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v.w[4 + i] = b[i];
   }
@@ -133,11 +134,16 @@ __device__ __forceinline__ Mx8<DT> mx_values8(uint32_t c, int e) {
   }
   return v;
 }
-template <int DT>
+template <int DT, bool ONCE = false>
 __device__ __forceinline__ void mx_store8(void* p, const Mx8<DT>& v) {
-  *reinterpret_cast<mx_v4u*>(p) = mx_v4u{v.w[0], v.w[1], v.w[2], v.w[3]};
-  if constexpr (DT == CDIT_DT_F32)
-    *(reinterpret_cast<mx_v4u*>(p) + 1) = mx_v4u{v.w[4], v.w[5], v.w[6], v.w[7]};
+  auto store = [](mx_v4u d, mx_v4u* q) {
+    if (ONCE)
+      __builtin_nontemporal_store(d, q);
+    else
+      *q = d;
+  };
+  store(mx_v4u{v.w[0], v.w[1], v.w[2], v.w[3]}, reinterpret_cast<mx_v4u*>(p));
+  if constexpr (DT == CDIT_DT_F32) store(mx_v4u{v.w[4], v.w[5], v.w[6], v.w[7]}, reinterpret_cast<mx_v4u*>(p) + 1);
 }
 
 // Eight codes as bf16, times their scale.
