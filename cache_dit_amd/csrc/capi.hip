@@ -639,10 +639,12 @@ static bool known_dtype(int id) { return id == CDIT_DT_F16 || id == CDIT_DT_BF16
 static int64_t mx_scale_bytes(int64_t K) { return (K + 127) / 128 * 4; }
 static bool on(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
+constexpr int64_t kMxMostK = (int64_t)1 << 29;  // (the quantizer's grid; offsets inside a row in 32 bits)
+
 // A matrix in MXFP4: codes on `align` bytes.
 static int check_mx(const char* fn, const char* what, const void* codes, const void* scales, int64_t rows, int64_t K,
                     int64_t ld_codes, int64_t ld_scales, int align) {
-  if (rows < 0 || K < 0 || rows > INT32_MAX || K > INT32_MAX - 512) {
+  if (rows < 0 || K < 0 || rows > INT32_MAX || K > kMxMostK) {
     set_error("%s: bad shape of %s (%lld x %lld)", fn, what, (long long)rows, (long long)K);
     return CDIT_EINVAL;
   }
@@ -710,7 +712,7 @@ int cdit_mxfp4_dequant(const void* codes, int64_t ld_codes, const void* scales, 
 }
 
 // What both 4-bit GEMMs ask of the weight and the output.
-static int check_mx_gemm(const char* fn, const void* w, const void* ws, const void* out, int64_t M, int64_t N, int64_t K,
+static int check_mx_gemm(const char* fn, const void* w, const void* ws, const void* bias, const void* out, int64_t M, int64_t N, int64_t K,
                          int64_t ldw, int64_t ldws, int64_t ldo, int epilogue, int out_dtype_id) {
   if (M < 0 || M > INT32_MAX - 512 || N > INT32_MAX - 512) {
     set_error("%s: bad shape (M=%lld N=%lld)", fn, (long long)M, (long long)N);
@@ -733,6 +735,11 @@ static int check_mx_gemm(const char* fn, const void* w, const void* ws, const vo
     set_error("%s: null pointer argument", fn);
     return CDIT_EINVAL;
   }
+  const int es = out_dtype_id == CDIT_DT_F32 ? 4 : 2;
+  if (!on(out, es) || !on(bias, es)) {
+    set_error("%s: misaligned pointer", fn);
+    return CDIT_EINVAL;
+  }
   return CDIT_OK;
 }
 
@@ -740,7 +747,7 @@ int cdit_mxfp4_gemm(const void* a_codes, const void* a_scales, const void* b_cod
                     void* out, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldas, int64_t ldb, int64_t ldbs,
                     int64_t ldo, int epilogue, int out_dtype_id, void* stream) {
   const char* fn = "cdit_mxfp4_gemm";
-  int rc = check_mx_gemm(fn, b_codes, b_scales, out, M, N, K, ldb, ldbs, ldo, epilogue, out_dtype_id);
+  int rc = check_mx_gemm(fn, b_codes, b_scales, bias, out, M, N, K, ldb, ldbs, ldo, epilogue, out_dtype_id);
   if (rc || (rc = check_mx(fn, "the activation", a_codes, a_scales, M, K, lda, ldas, 16))) return rc;
   if (M == 0 || N == 0) return CDIT_OK;
   if ((rc = check_arch())) return rc;
@@ -755,9 +762,9 @@ int cdit_mxfp4_linear(const void* x_bf16, const void* w_codes, const void* w_sca
                       void* codes_ws, void* scales_ws, int64_t M, int64_t N, int64_t K, int64_t ld_x, int64_t ldw,
                       int64_t ldws, int64_t ldo, int epilogue, void* stream) {
   const char* fn = "cdit_mxfp4_linear";
-  int rc = check_mx_gemm(fn, w_codes, w_scales, out, M, N, K, ldw, ldws, ldo, epilogue, CDIT_DT_BF16);
+  int rc = check_mx_gemm(fn, w_codes, w_scales, bias_bf16, out, M, N, K, ldw, ldws, ldo, epilogue, CDIT_DT_BF16);
   if (rc || (rc = check_mx(fn, "the workspaces", codes_ws, scales_ws, M, K, K / 2, mx_scale_bytes(K), 16))) return rc;
-  if (g_gemm_variant < 0 && N > 0 && mx_rows_fit(false, (int)M, (int)N)) {  // few rows: one kernel that quantizes them itself
+  if (g_gemm_variant < 0 && N > 0 && mx_rows_fit(false, M, N, ldw)) {  // few rows: one kernel that quantizes them itself
     if ((rc = check_mx_dense(fn, x_bf16, M, K, ld_x, CDIT_DT_BF16)) || (rc = check_arch())) return rc;
     const Mx4Gemm g{static_cast<const uint8_t*>(x_bf16), nullptr, static_cast<const uint8_t*>(w_codes),
                     static_cast<const uint8_t*>(w_scales), bias_bf16, out, (int)M, (int)N, (int)K, ld_x, 0, ldw, ldws, ldo,
@@ -775,7 +782,7 @@ int cdit_w4a16_gemm(const void* x_bf16, const void* w_codes, const void* w_scale
                     int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldw, int64_t ldws, int64_t ldo, int epilogue,
                     void* stream) {
   const char* fn = "cdit_w4a16_gemm";
-  int rc = check_mx_gemm(fn, w_codes, w_scales, out, M, N, K, ldw, ldws, ldo, epilogue, CDIT_DT_BF16);
+  int rc = check_mx_gemm(fn, w_codes, w_scales, bias_bf16, out, M, N, K, ldw, ldws, ldo, epilogue, CDIT_DT_BF16);
   if (rc || (rc = check_mx_dense(fn, x_bf16, M, K, lda, CDIT_DT_BF16))) return rc;
   if (M == 0 || N == 0) return CDIT_OK;
   if ((rc = check_arch())) return rc;

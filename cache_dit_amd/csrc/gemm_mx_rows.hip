@@ -234,9 +234,11 @@ int launch_rows(const Mx4Gemm& g, hipStream_t stream) {
 // time grows with rows times columns; us, this kernel and the best tile (w4a4 with its quantizer), M x N x K, weights from HBM:
 // w4a4 4 x 13824 x 5120 14.9 and 18.1, 8: 17.1 and 18.5, 16: 21.2 and 18.2; 16 x 5120 x 5120 14.0 and 14.8; 16 x 30720 x 5120 38.8
 // and 25.5. Weight-only 8 x 13824 x 5120 17.9 and 24.4, 16: 23.7 and 25.1; 16 x 30720 x 5120 45.9 and 32.4.
-bool mx_rows_fit(bool weight_only, int M, int N) {
-  return M >= 1 && M <= 16 && (int64_t)M * ((N + 15) / 16) < (weight_only ? 20000 : 10000);
+bool mx_rows_fit(bool weight_only, int64_t M, int64_t N, int64_t ldb) {
+  return mx_rows_can(M, ldb) && M * ((N + 15) / 16) < (weight_only ? 20000 : 10000);
 }
+// Whether it can take them: 16 rows of the activation, and of the weight 16 within 32-bit offsets.
+bool mx_rows_can(int64_t M, int64_t ldb) { return M >= 1 && M <= 16 && ldb < (int64_t)1 << 27; }
 
 int launch_gemm_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream) { return launch_rows<kCodes>(g, stream); }
 int launch_linear_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream) { return launch_rows<kQuantize, CDIT_DT_BF16>(g, stream); }

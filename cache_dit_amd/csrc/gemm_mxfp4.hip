@@ -391,14 +391,14 @@ static const MxTime kTimes[] = {
     {4, 64, 64, 2500, 1060, 319, 235},      {8, 32, 64, 2500, 850, 294, 174}};
 
 int choose_gemm_mxfp4(const Mx4Gemm& g) {
-  if (mx_rows_fit(false, g.M, g.N)) return kMxRows;
+  if (mx_rows_fit(false, g.M, g.N, g.ldb)) return kMxRows;
   const int cus = cu_count();
   return tiles_fit(g, 1) ? fastest_tile(kTimes, sizeof(kTimes) / sizeof(kTimes[0]), g, cus > 0 ? cus : 256) : 0;
 }
 
 int launch_gemm_mxfp4(const Mx4Gemm& g, int variant, hipStream_t stream) {
   if (variant < 0) variant = choose_gemm_mxfp4(g);
-  if (variant == kMxRows && g.M <= 16) return launch_gemm_mxfp4_rows(g, stream);
+  if (variant == kMxRows && mx_rows_can(g.M, g.ldb)) return launch_gemm_mxfp4_rows(g, stream);
   if (!tiles_fit(g, 1)) variant = 0;
   if (variant == 1 && g.out_dtype == CDIT_DT_F32) variant = 5;  // (no registers left for 16-byte stores of 256 x 256)
   switch (variant) {

@@ -503,14 +503,14 @@ static const MxTime kTimes[] = {
     {4, 64, 64, 2300, 900, 1000, 681},      {8, 32, 64, 1800, 1200, 780, 836}};
 
 int choose_gemm_w4a16(const Mx4Gemm& g) {
-  if (mx_rows_fit(true, g.M, g.N)) return kMxRows;
+  if (mx_rows_fit(true, g.M, g.N, g.ldb)) return kMxRows;
   const int cus = cu_count();
   return tiles_fit(g, 2) ? fastest_tile(kTimes, sizeof(kTimes) / sizeof(kTimes[0]), g, cus > 0 ? cus : 256) : 0;
 }
 
 int launch_gemm_w4a16(const Mx4Gemm& g, int variant, hipStream_t stream) {
   if (variant < 0) variant = choose_gemm_w4a16(g);
-  if (variant == kMxRows && g.M <= 16) return launch_gemm_w4a16_rows(g, stream);
+  if (variant == kMxRows && mx_rows_can(g.M, g.ldb)) return launch_gemm_w4a16_rows(g, stream);
   if (!tiles_fit(g, 2)) variant = 0;
   switch (variant) {
     case 1: return launch_tile<W4Tile<256, 256, 2, 2, 3, 1>>(g, stream);

@@ -608,7 +608,7 @@ at::ScalarType dtype_of(int64_t id) { return id == CDIT_DT_F16 ? at::kHalf : id 
 // contiguous tensor, a slice [:, n:] of one batch entry.
 bool even_rows(const at::Tensor& t, Rows* r) {
   const int64_t d = t.dim();
-  if (d < 1 || t.size(d - 1) <= 0 || t.stride(d - 1) != 1) return false;
+  if (d < 1 || t.size(d - 1) <= 0 || (t.stride(d - 1) != 1 && t.size(d - 1) > 1)) return false;
   r->K = t.size(d - 1);
   r->M = 1;
   r->ld = r->K;
@@ -634,6 +634,8 @@ struct MxRows {
 };
 bool mx_rows(const at::Tensor& codes, const at::Tensor& scales, int align, MxRows* m) {
   Rows c, s;
+  if (codes.dim() < 1 || codes.dim() != scales.dim() || codes.sizes().slice(0, codes.dim() - 1) != scales.sizes().slice(0, codes.dim() - 1))
+    return false;
   if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kByte || !even_rows(codes, &c) || !even_rows(scales, &s) ||
       c.M <= 0 || s.M != c.M || c.K % 16 || s.K != mx_scale_bytes(2 * c.K) || c.ld < c.K || s.ld < s.K || c.ld % align ||
       s.ld % 4 || reinterpret_cast<uintptr_t>(codes.data_ptr()) % align ||
@@ -757,7 +759,7 @@ PyObject* gate_residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int type = dtype_id(t.scalar_type());
     const bool f32 = type == CDIT_DT_F32 && g.dtype != CDIT_DT_F32;
     const int64_t d = t.dim(), count = g.K > 0 ? t.numel() / g.K : 0;
-    plain = d >= 1 && t.size(d - 1) == g.K && t.stride(d - 1) == 1 && (type == g.dtype || f32) && t.device() == x.device() &&
+    plain = d >= 1 && t.size(d - 1) == g.K && (t.stride(d - 1) == 1 || g.K == 1) && (type == g.dtype || f32) && t.device() == x.device() &&
             (!any || f32 == (g.vec_f32 != 0)) && count >= 1;
     if (!plain) return;
     any = true;

@@ -161,7 +161,7 @@ def _bias_vector(bias: Optional[torch.Tensor], dtype: torch.dtype) -> Optional[t
   return bias if bias.data_ptr() % 16 == 0 else bias.clone()
 
 
-def _empty_product(rows: torch.Tensor, N: int, dtype: torch.dtype, K: int, bias, epilogue: int) -> torch.Tensor:
+def _empty_product(rows: torch.Tensor, N: int, dtype: torch.dtype, bias, epilogue: int) -> torch.Tensor:
   """What a product without rows, columns or a sum is: the epilogue of the bias."""
   out = torch.zeros((*rows.shape[:-1], N), dtype=torch.float32, device=rows.device)
   if bias is not None:
@@ -182,7 +182,7 @@ def _mxfp4_mm(a_codes, a_scales, b_codes, b_scales, bias, out_dtype_id, epilogue
   K = _check_mx(name, "the activation", a_codes, a_scales)
   N = _check_weight(name, K, b_codes, b_scales, bias, a_codes)
   if K == 0 or N == 0 or a_codes.numel() == 0:
-    return _empty_product(a_codes, N, out_dtype, K, bias, epilogue)
+    return _empty_product(a_codes, N, out_dtype, bias, epilogue)
   out = _results(host.mxfp4_mm(_aligned_rows(a_codes, 16), _aligned_rows(a_scales, 4), _aligned_rows(b_codes, 16),
                                _aligned_rows(b_scales, 4), _bias_vector(bias, out_dtype), out_dtype_id, epilogue))[0]
   return _shaped(out, *a_codes.shape[:-1], N)
@@ -205,7 +205,7 @@ def _linear(name, launch, x, weight, weight_scale, bias, epilogue):
   _check_k(name, x.shape[-1])
   N = _check_weight(name, x.shape[-1], weight, weight_scale, bias, x)
   if N == 0 or x.numel() == 0:
-    return _empty_product(x, N, torch.bfloat16, x.shape[-1], bias, epilogue)
+    return _empty_product(x, N, torch.bfloat16, bias, epilogue)
   out = _results(launch(_aligned_rows(x, 16), _aligned_rows(weight, 16), _aligned_rows(weight_scale, 4),
                         _bias_vector(bias, torch.bfloat16), epilogue))[0]
   return _shaped(out, *x.shape[:-1], N)

@@ -364,8 +364,9 @@ int cdit_fp8_linear_w8a8_static(const void* x_bf16, const void* w_q, const float
  * codes  uint8 [M, K/2]: element 2j in the low half of byte j, 2j + 1 in the high half; bit 3 the sign, bits 0..2 the
  *        magnitude 0, .5, 1, 1.5, 2, 3, 4, 6.
  * scales uint8 [M, 4 ceil(K/128)]: byte b is the scale 2^(s - 127) of elements 32 b .. 32 b + 31, 255 a NaN; the up to
- *        three bytes behind K/32 are 127. (For K a multiple of 128 that is [M, K/32] without padding.)
- * K is a multiple of 32. Leading dimensions of codes and scales are in bytes; rows of codes start on a multiple of 4
+ *        three bytes behind K/32 are 127. (For K a multiple of 128 that is [M, K/32] without padding. The GEMMs multiply
+ *        zeros under the scales behind K/32: a 255 there makes the row NaN.)
+ * K is a multiple of 32, 2^29 at most. Leading dimensions of codes and scales are in bytes; rows of codes start on a multiple of 4
  * bytes for the quantizer and its inverse, of 16 for the GEMMs; rows of scales on a multiple of 4.
  *
  * cdit_mxfp4_quant: x [M,K] (ld_x in elements, rows on 16 bytes) of x_dtype_id ->
