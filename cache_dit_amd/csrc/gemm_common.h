@@ -74,12 +74,12 @@ __device__ __forceinline__ void store_out(const GemmArgs& g, int64_t idx, float 
 // folded: 3 multiplies, 1 FMA, 1 add and the two transcendental instructions per
 // element. exp2 overflow gives v * 0 = -0 for very negative v and exp2 underflow
 // gives v * 1 for very positive v, the correct limits.
-__device__ __forceinline__ float gelu_tanh(float v) {
+__device__ __forceinline__ float gelu_exp(float v) {  // exp(-2u)
   const float kC0 = -2.302208198f;    // -2 log2(e) sqrt(2/pi)
   const float kC1 = -0.10294323958f;  // kC0 * 0.044715
-  const float e = __builtin_amdgcn_exp2f(v * __fmaf_rn(v * v, kC1, kC0));
-  return v * __builtin_amdgcn_rcpf(1.0f + e);
+  return __builtin_amdgcn_exp2f(v * __fmaf_rn(v * v, kC1, kC0));
 }
+__device__ __forceinline__ float gelu_tanh(float v) { return v * __builtin_amdgcn_rcpf(1.0f + gelu_exp(v)); }
 
 // Eight e4m3 values (two words) as bf16, exact. Not for operands of inline-assembly MFMAs.
 __device__ __forceinline__ v8bf e4m3x8_to_bf16(uint32_t lo, uint32_t hi) {

@@ -386,7 +386,7 @@ int launch_tile(const Mx4Gemm& g, hipStream_t stream) {
 
 // Times from problems of a quarter of a round to eight rounds at K = 1024 and 5120.
 static const MxTime kTimes[] = {
-    {1, 256, 256, 10000, 6100, 1790, 1900}, {5, 128, 256, 3500, 2700, 1070, 1117}, {6, 256, 128, 3500, 2700, 1070, 1117},
+    {1, 256, 256, 8000, 2800, 1880, 1890}, {5, 128, 256, 3500, 2700, 1070, 1117}, {6, 256, 128, 3500, 2700, 1070, 1117},
     {2, 128, 128, 2700, 1000, 610, 579},    {3, 64, 128, 2700, 900, 430, 372},     {7, 128, 64, 2700, 1000, 412, 360},
     {4, 64, 64, 2500, 1060, 319, 235},      {8, 32, 64, 2500, 850, 294, 174}};
 

@@ -498,7 +498,7 @@ int launch_split(const Mx4Gemm& g, hipStream_t stream) {
 
 // Times from problems of a quarter of a round to eight rounds at K = 1024 and 5120.
 static const MxTime kTimes[] = {
-    {1, 256, 256, 3500, 15800, 5775, 5300}, {5, 128, 256, 2700, 2750, 3575, 3190}, {6, 256, 128, 2700, 3000, 3510, 3040},
+    {1, 256, 256, 3500, 4400, 5880, 5580}, {5, 128, 256, 2700, 2750, 3575, 3190}, {6, 256, 128, 2700, 3000, 3510, 3040},
     {2, 128, 128, 2700, 900, 1940, 1750},   {3, 64, 128, 2700, 700, 1380, 1090},   {7, 128, 64, 2700, 700, 1220, 1150},
     {4, 64, 64, 2300, 900, 1000, 681},      {8, 32, 64, 1800, 1200, 780, 836}};
 

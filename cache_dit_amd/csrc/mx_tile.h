@@ -69,18 +69,39 @@ __device__ __forceinline__ void store_mx_tile(v16f (&acc)[TM][TN], const Mx4Gemm
   const uint32_t off = (uint32_t)row * row_bytes + (uint32_t)n * OB;
   const bool cut = g.N % TN != 0 && __builtin_amdgcn_readfirstlane(n) + 32 * TN > g.N;  // (a wavefront's first lane: its first column)
   constexpr int kStoreOnce = 2;  // non-temporal: whole lines, written once
-  auto store = [&](auto gelu_tag) {
+  // The 256 x 256 tile has its sums in accumulation registers. Left to itself the compiler copies them to others ahead of the
+  // stores, many of them several times, and spills for it: here each is read where it is stored. The wait covers the last
+  // matrix instruction, which the compiler does not see these reads depend on. us, without and with: w4a4 32760 x 13824 x 5120
+  // 1160 and 1080, 8192 x 10240 x 2560 134 and 118, with GELU (and its steps in order, below) 166 and 128; w4a16 16384 x 5120 x
+  // 5120 630 and 592. The tiles of half the size keep theirs where the compiler puts them: 1230 either way.
+  constexpr bool IN_AGPRS = TM * TN >= 16;
+  if constexpr (IN_AGPRS) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  }
+  auto store = [&](auto gelu_tag, auto cut_tag) {
     const int at = (int)(n + TN <= g.N ? off : 0x80000000u);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const uint32_t at_row = (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3)) * row_bytes;
-        float v[TN];
+        float v[TN], ex[TN];
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          v[j] = acc[i][j][e];
-          if constexpr (decltype(gelu_tag)::value) v[j] = gelu_tanh(v[j]);
+          if constexpr (IN_AGPRS)
+            asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[j]) : "a"(acc[i][j][e]));
+          else
+            v[j] = acc[i][j][e];
+        }
+        if constexpr (decltype(gelu_tag)::value) {
+          // (step by step: one wavefront a SIMD, and nothing but the other columns covers the latency of a step)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) ex[j] = gelu_exp(v[j]);
+          if constexpr (IN_AGPRS) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) v[j] *= __builtin_amdgcn_rcpf(1.0f + ex[j]);
+          if constexpr (IN_AGPRS) __builtin_amdgcn_sched_barrier(0);
         }
         auto pack = [](float lo, float hi) -> uint32_t {
           return OUT == CDIT_DT_F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
@@ -102,27 +123,32 @@ __device__ __forceinline__ void store_mx_tile(v16f (&acc)[TM][TN], const Mx4Gemm
           const short d = (short)w[0];
           __builtin_amdgcn_raw_buffer_store_b16(d, out, at, at_row, kStoreOnce);
         }
-        if constexpr (TN > 1) {
-          if (cut) {
+        if constexpr (decltype(cut_tag)::value) {
 #pragma unroll
-            for (int j = 0; j < TN - 1; ++j) {
-              const int one = (int)(n + TN > g.N && n + j < g.N ? off + j * OB : 0x80000000u);
-              if constexpr (OUT == CDIT_DT_F32) {
-                const uint32_t d = w[j];
-                __builtin_amdgcn_raw_buffer_store_b32(d, out, one, at_row, 0);
-              } else {
-                const short d = (short)(w[j & ~1] >> (16 * (j & 1)));
-                __builtin_amdgcn_raw_buffer_store_b16(d, out, one, at_row, 0);
-              }
+          for (int j = 0; j < TN - 1; ++j) {
+            const int one = (int)(n + TN > g.N && n + j < g.N ? off + j * OB : 0x80000000u);
+            if constexpr (OUT == CDIT_DT_F32) {
+              const uint32_t d = w[j];
+              __builtin_amdgcn_raw_buffer_store_b32(d, out, one, at_row, 0);
+            } else {
+              const short d = (short)(w[j & ~1] >> (16 * (j & 1)));
+              __builtin_amdgcn_raw_buffer_store_b16(d, out, one, at_row, 0);
             }
           }
         }
       }
   };
+  // (a branch around all of the stores, not one in each of them)
+  auto store_cut = [&](auto gelu_tag) {
+    if constexpr (TN > 1) {
+      if (cut) return store(gelu_tag, std::true_type{});
+    }
+    store(gelu_tag, std::false_type{});
+  };
   if (g.epilogue & CDIT_EPI_GELU_TANH)
-    store(std::true_type{});
+    store_cut(std::true_type{});
   else
-    store(std::false_type{});
+    store_cut(std::false_type{});
 }
 
 }  // namespace
