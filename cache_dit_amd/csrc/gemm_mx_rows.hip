@@ -4,7 +4,8 @@
 // quantized on the way where the caller has it in bf16. K is split between the W wavefronts in items of 512; a wavefront reads an
 // item's weights straight from memory (every byte is used once, the next item's loads are under way meanwhile) and multiplies
 // them with the activation's rows on the matrix core, and the W partial sums of 16 x 16 outputs meet in LDS. Bound by HBM, and
-// by latency where N is small.
+// by latency where N is small: 1 x 30720 x 5120 (M x N x K) 17.9 us for 84 MB, where a kernel that only reads them takes 14.8; 1 x
+// 13824 x 5120 10.8 with the weight in the caches as far as it fits, 12.8 from HBM (8.2 to only read it).
 //
 // Lane l is row l & 15 (a column of the output; a row of the activation) and K block l >> 4 of a step of 128: 16 bytes of codes,
 // 64 of each row in a request, and the scale in byte l >> 4 of the step's word. The scales go through LDS: 16 rows of them are

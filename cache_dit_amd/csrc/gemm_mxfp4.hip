@@ -18,7 +18,7 @@ __device__ __forceinline__ v4f mfma_mx(v4i w, v4i a, v4f acc, int w_scale, int a
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, a8, acc, 4, 4, 0, w_scale, 0, a_scale);
 }
 
-// A wavefront per 32 x 32 outputs, operands straight from memory.
+// A wavefront per 32 x 32 outputs, operands straight from memory: any stride (the tiles below address with 32 bits).
 template <int OUT>
 __global__ __launch_bounds__(256) void gemm_mxfp4_direct(Mx4Gemm g) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
@@ -85,6 +85,13 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_direct(Mx4Gemm g) {
 // Scales: a lane needs bytes 2 j + (l >> 5) of its row for the rounds j = 0 .. 15 of 1024 along K. It loads 16 of those 32 bytes
 // (those of its own half; a row's 32 are one request), and byte permutations and a swap between the halves of the
 // wavefront bring them in order.
+//
+// Measured (M x N x K, weights and codes in HBM or caches as they come): 32760 x 13824 x 5120 in 256 x 256 tiles 1080 us, 4.29
+// PFLOP/s; a loop of nothing but the instruction on random operands runs at 6.4 (the clock falls to 1.56 GHz), 725 us. Matrix cores
+// busy 65 % of the cycles, no LDS conflicts. With a part left out: no scales after a tile's first 1050, no LDS-DMA after three
+// steps 1110, no LDS reads 1045, no stores 1040, none of scales, DMA and reads 945: a wavefront a SIMD has nothing to cover a
+// tile's end (2.8 us) and a step's changes with. Two a SIMD (128 x 256) need 1.7 times the reads per product: 1225 us. Few tiles
+// are bound by what a CU takes from the caches, 50 to 60 GB/s: 512 x 5120 x 4096 in 128 x 128 tiles (160 of 256 CUs) 13.9 us.
 template <int BM_, int BN_, int WGM_, int WGN_, int SA_, int SB_, int WPE_>
 struct MxTile {
   static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, SA = SA_, SB = SB_, WPE = WPE_;

@@ -16,7 +16,7 @@ namespace {
 // The scale of a block as the converter takes it; NaN for a NaN block.
 __device__ __forceinline__ float mx_weight_scale(int e) { return e == kMxNan ? __uint_as_float(0x7fc00000u) : mx_scale_f32(e); }
 
-// A wavefront per 32 x 32 outputs, operands straight from memory.
+// A wavefront per 32 x 32 outputs, operands straight from memory: any stride (the tiles below address with 32 bits).
 __global__ __launch_bounds__(256) void gemm_w4a16_direct(Mx4Gemm g) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
   const int n0 = blockIdx.x * 128 + wave * 32;
@@ -83,6 +83,9 @@ __global__ __launch_bounds__(256) void gemm_w4a16_direct(Mx4Gemm g) {
 //   q = 3: MFMAs; meanwhile codes and first fragments of step x + 1 are read, and converted
 //   DMA of X's step x + SA from here to the end of the next step's q = 2; of the weight's line k + SB in the first two steps of
 //   line k + 1 (the codes of a line are read one step ahead)
+//
+// Measured: 4608 x 5120 x 5120 (M x N x K) 190 us, 1.27 PFLOP/s, 16384 x 5120 x 5120 592 us, 1.45 (256 x 256 tiles); the
+// library's bf16 product reaches 1.36 on 16384 x 16384 x 16384. Bound by the matrix cores at the clock they run at.
 template <int BM_, int BN_, int WGM_, int WGN_, int SA_, int WPE_>
 struct W4Tile {
   static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, SA = SA_, SB = 2, WPE = WPE_;
