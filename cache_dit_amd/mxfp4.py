@@ -260,6 +260,7 @@ def _norm_vector(name, what, t, x, dtype, per_row):
 
 def _gate_residual_norm_general(name, x, branch, gate, shift, scale, norm_weight, post_weight, norm, post_norm,
                                 residual_scale, eps, codes):
+  _reject_codes_only(name, x, branch)
   launch = _native.host().gate_residual_norm
   launched = launch(x, branch, gate, shift, scale, norm_weight, post_weight, norm, post_norm, residual_scale, eps, codes)
   if launched is not None:
@@ -398,7 +399,6 @@ def gate_residual_norm(x: torch.Tensor, branch: torch.Tensor, gate: Optional[tor
     raise ValueError(f"{name}: quant_type must be None or 'mxfp4', got {quant_type!r}")
   if not eps >= 0:
     raise ValueError(f"{name}: eps must not be negative, got {eps}")
-  _reject_codes_only(name, x, branch)
   op = _norm_op if quant_type is None else _norm_mxfp4_op
   return op(x, branch, gate, shift, scale, norm_weight, post_weight, NORM_IDS[norm], NORM_IDS[post_norm],
             float(residual_scale), float(eps))

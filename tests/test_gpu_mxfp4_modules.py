@@ -280,6 +280,9 @@ def test_compiled_module(cd, qt, M):
     x3 = rand(2, M, 96, seed=5)
     assert torch.equal(compiled(x3), net(x3))
 
+    # (an activation of which only FP8 codes exist must not stop the tracing of other calls)
+    only_codes = cd.ln_modulate_quant(rand(M, 128, seed=8), rand(128, seed=9), rand(128, seed=10), materialize=False)
+
     def norm(x, b, g):
       return cd.gate_residual_norm(x, b, g, norm="rms", quant_type="mxfp4")
 
@@ -287,6 +290,9 @@ def test_compiled_module(cd, qt, M):
     for got, want in zip(torch.compile(norm, fullgraph=True)(x, b, g), norm(x, b, g)):
       assert torch.equal(got, want)
   torch._dynamo.reset()
+  for call in (lambda: norm(only_codes, only_codes, None), lambda: cd.mxfp4_quant(only_codes)):
+    with pytest.raises(RuntimeError, match="codes only"):
+      call()
 
 
 def test_forms_that_layouts_may_take(cd):
