@@ -66,7 +66,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void gemm_mx_rows(Mx4Gemm g, int G
     for (int s = 0; s < 4; ++s) {
       const int e = ws[4 * s];
       if constexpr (MODE == kWeightOnly) {
-        const float f = e == kMxNan ? __uint_as_float(0x7fc00000u) : mx_scale_f32(e);
+        const float f = mx_scale_or_nan(e);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           acc[q & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_to_bf16(w.c[s][q], f),

@@ -13,9 +13,6 @@
 namespace cdit {
 namespace {
 
-// The scale of a block as the converter takes it; NaN for a NaN block.
-__device__ __forceinline__ float mx_weight_scale(int e) { return e == kMxNan ? __uint_as_float(0x7fc00000u) : mx_scale_f32(e); }
-
 // A wavefront per 32 x 32 outputs, operands straight from memory: any stride (the tiles below address with 32 bits).
 __global__ __launch_bounds__(256) void gemm_w4a16_direct(Mx4Gemm g) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kg = lane >> 4;
@@ -45,7 +42,7 @@ __global__ __launch_bounds__(256) void gemm_w4a16_direct(Mx4Gemm g) {
           av[i][q] = __builtin_bit_cast(v8bf, in ? *reinterpret_cast<const v4u*>(a[i] + 256 * (int64_t)s + 16 * q) : z);
         }
         wv[i] = in ? *reinterpret_cast<const v4u*>(w[i] + 64 * (int64_t)s) : v4u{0, 0, 0, 0};
-        wsv[i] = in ? mx_weight_scale(ws[i][4 * s]) : 1.0f;
+        wsv[i] = in ? mx_scale_or_nan(ws[i][4 * s]) : 1.0f;
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q)
@@ -63,11 +60,7 @@ __global__ __launch_bounds__(256) void gemm_w4a16_direct(Mx4Gemm g) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int m = m0 + 16 * i + r, n = n0 + 16 * j + 4 * kg + e;
-          if (m >= g.M || n >= g.N) continue;
-          float v = acc[i][j][e];
-          if (g.bias) v += bias_to_f32<CDIT_DT_BF16>(static_cast<const uint16_t*>(g.bias)[n]);
-          if (g.epilogue & CDIT_EPI_GELU_TANH) v = gelu_tanh(v);
-          static_cast<uint16_t*>(g.out)[(int64_t)m * g.ldo + n] = (uint16_t)f32_to_bf16_bits(v);
+          if (m < g.M && n < g.N) store_mx_one<CDIT_DT_BF16>(g, m, n, acc[i][j][e]);
         }
   }
 }
@@ -220,10 +213,7 @@ gemm_w4a16_tile(Mx4Gemm g, int tiles_m, int tiles_n) {
   v4u a[2][TM], wc[2][TN];  // X's fragments by q, codes by step
   v8bf wb[2][TN];           // converted, by q
   float fs[2][TN];          // scales by step
-  auto scale_of = [&](uint32_t bytes, int t) -> float {
-    const int e = (bytes >> (8 * t)) & 255;
-    return e == kMxNan ? __uint_as_float(0x7fc00000u) : mx_scale_f32(e);
-  };
+  auto scale_of = [&](uint32_t bytes, int t) -> float { return mx_scale_or_nan((bytes >> (8 * t)) & 255); };
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
     wc[0][j] = read(smem + b_cur, rd_b[0], j);
@@ -456,8 +446,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_w4a16_split(Mx4Gemm g, int ti
     v4u a[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) a[q] = read(smem + stage, rd_a + (((4 * h + q) ^ swz) << 4));
-    const int e = (sc >> (8 * (2 * (grp & 1) + h))) & 255;
-    const float f = e == kMxNan ? __uint_as_float(0x7fc00000u) : mx_scale_f32(e);
+    const float f = mx_scale_or_nan((sc >> (8 * (2 * (grp & 1) + h))) & 255);
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a[q]), mx_to_bf16(c[q], f), acc, 0, 0, 0);

@@ -38,6 +38,9 @@ __device__ __forceinline__ int mx_exponent(uint32_t amax_bits) {
 // 2^(e - 127) as the converters take it: they read the exponent bits alone.
 __device__ __forceinline__ float mx_scale_f32(int e) { return __uint_as_float((uint32_t)e << 23); }
 
+// The same, NaN for a block that is not finite.
+__device__ __forceinline__ float mx_scale_or_nan(int e) { return e == kMxNan ? __uint_as_float(0x7fc00000u) : mx_scale_f32(e); }
+
 // Eight consecutive elements as they lie in memory (four words of 16-bit types, eight of fp32).
 template <int DT>
 struct Mx8 {

@@ -423,3 +423,95 @@ def test_strides_beyond_32_bits(cd, qt):
   for M in (1, 16, 100):
     x = rand(M, K, seed=M)
     check_product(f(x, wide[:, :K // 2], scales), x, codes, scales, None, qt)
+
+
+# ------------------------------------------------------------------------- C interface
+
+
+def framed(rows, row_bytes, ld_bytes):
+  """Memory of 0x5a with room for `rows` rows, 64 bytes in front, one row and 64 bytes behind; the rows' view."""
+  m = torch.full((64 + (rows + 1) * ld_bytes + 64, ), 0x5a, dtype=torch.uint8, device="cuda")
+  return m, m[64:64 + rows * ld_bytes].view(rows, ld_bytes)[:, :row_bytes]
+
+
+def rest_is_untouched(m, view):
+  view.fill_(0x5a)
+  assert (m == 0x5a).all()
+
+
+@pytest.mark.parametrize("v", [-1, 0, 1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("M,N,K", [(1, 77, 96), (13, 33, 544), (70, 131, 160), (300, 260, 512)])
+def test_nothing_but_the_outputs_is_written(cd, variant, v, M, N, K):
+  """Outputs, codes, scales and workspaces with rows further apart than they are long, in memory that is looked over."""
+  from cache_dit_amd import _native
+  lib, stream = _native.load(), torch.cuda.current_stream().cuda_stream
+  S = mo.scale_bytes(K)
+  x, w, bias = rand(M, K, seed=1), rand(N, K, seed=2, std=0.05), rand(N, seed=3, std=0.1)
+  codes, scales = cd.mxfp4_quant(w)
+  a, a_s = cd.mxfp4_quant(x)
+  variant(v)
+  want = [cd.ops.mxfp4_linear(x, codes, scales, bias), cd.ops.w4a16_mm(x, codes, scales, bias),
+          cd.mxfp4_mm(a, a_s, codes, scales, BF16, bias)]
+
+  def call(f, *args):
+    assert f(*args) == 0, lib.cdit_last_error()
+    torch.cuda.synchronize()
+
+  ldo = N + 5
+  for which in range(3):
+    m, out = framed(M, 2 * N, 2 * ldo)
+    mq, q = framed(M, K // 2, K // 2)
+    ms, s = framed(M, S, S)
+    p = [codes.data_ptr(), scales.data_ptr(), bias.data_ptr(), out.data_ptr()]
+    if which == 0:
+      call(lib.cdit_mxfp4_linear, x.data_ptr(), *p, q.data_ptr(), s.data_ptr(), M, N, K, K, K // 2, S, ldo, 0, stream)
+    elif which == 1:
+      call(lib.cdit_w4a16_gemm, x.data_ptr(), *p, M, N, K, K, K // 2, S, ldo, 0, stream)
+    else:
+      call(lib.cdit_mxfp4_gemm, a.data_ptr(), a_s.data_ptr(), *p, M, N, K, K // 2, S, K // 2, S, ldo, 0, 1, stream)
+    assert torch.equal(out.contiguous().view(BF16), want[which]), which
+    for memory, view in ((m, out), (mq, q), (ms, s)):
+      rest_is_untouched(memory, view)
+  if v != -1:
+    return
+  mq, q = framed(M, K // 2, K // 2 + 20)
+  ms, s = framed(M, S, S + 8)
+  call(lib.cdit_mxfp4_quant, x.data_ptr(), 1, M, K, K, q.data_ptr(), K // 2 + 20, s.data_ptr(), S + 8, stream)
+  assert torch.equal(q, a) and torch.equal(s, a_s)
+  md, d = framed(M, 2 * K, 2 * K + 48)
+  call(lib.cdit_mxfp4_dequant, q.data_ptr(), K // 2 + 20, s.data_ptr(), S + 8, M, K, d.data_ptr(), 1, K + 24, stream)
+  assert torch.equal(d.contiguous().view(BF16), cd.mxfp4_dequant(a, a_s))
+  for memory, view in ((mq, q), (ms, s), (md, d)):
+    rest_is_untouched(memory, view)
+
+
+@pytest.mark.parametrize("K,gap", [(96, 8), (96, 3), (1000, 8), (5120, 24), (12288, 8), (16416, 8)])
+@pytest.mark.parametrize("codes", [False, True])
+def test_nothing_but_the_norm_is_written(cd, K, gap, codes):
+  import ctypes
+
+  from cache_dit_amd import _native
+  from test_mxfp4_cpu import NormArgs
+  if codes and K % 32:
+    pytest.skip("codes need whole blocks")
+  lib, stream, M = _native.load(), torch.cuda.current_stream().cuda_stream, 7
+  x, b, g = rand(M, K, seed=1), rand(M, K, seed=2), rand(K, seed=3)
+  ld, S = K + gap, mo.scale_bytes(K)
+  (mh, h), (my, y) = framed(M, 2 * K, 2 * ld), framed(M, 2 * K, 2 * ld)
+  (mq, q), (ms, s) = framed(M, K // 2, K // 2 + 4), framed(M, S, S + 4)
+  args = NormArgs(M=M, K=K, x=x.data_ptr(), ld_x=K, branch=b.data_ptr(), ld_branch=K, x_dtype=1, dtype=1, gate=g.data_ptr(),
+                  ld_gate=0, rows_per_gate=M, norm=2, residual_scale=1.0, eps=1e-6, h=h.data_ptr(), ld_h=ld, y=y.data_ptr(),
+                  ld_y=ld)
+  if codes:
+    args.codes, args.ld_codes, args.code_scales, args.ld_code_scales = q.data_ptr(), K // 2 + 4, s.data_ptr(), S + 4
+  assert lib.cdit_gate_residual_norm(ctypes.byref(args), stream) == 0, lib.cdit_last_error()
+  torch.cuda.synchronize()
+  want = cd.gate_residual_norm(x, b, g, norm="rms")
+  assert torch.equal(h.contiguous().view(BF16), want[0])
+  got = y.contiguous().view(BF16)
+  # (rows off 16 bytes take the kernel that reads them again: another order of additions, a step of bf16 here and there)
+  assert (got.float() - want[1].float()).abs().max() <= 2.0**-7 * want[1].float().abs().max()
+  if codes:
+    assert all(torch.equal(t, u) for t, u in zip((q, s), cd.mxfp4_quant(got)))
+  for memory, view in ((mh, h), (my, y), (mq, q), (ms, s)):
+    rest_is_untouched(memory, view)
