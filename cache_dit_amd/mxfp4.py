@@ -386,10 +386,13 @@ def gate_residual_norm(x: torch.Tensor, branch: torch.Tensor, gate: Optional[tor
   The reference runs these as separate tensor operations in the blocks it patches
   (src/cache_dit/caching/patch_functors/functor_flux.py:48-80)."""
   name = "gate_residual_norm"
-  tensors = (x, branch, gate, shift, scale, norm_weight, post_weight)
-  _require_cuda(name, *tensors)
-  if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-    raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad()")
+  grad = torch.is_grad_enabled()
+  for t in (x, branch, gate, shift, scale, norm_weight, post_weight):
+    if t is not None:
+      if not t.is_cuda:
+        _require_cuda(name, t)
+      if grad and t.requires_grad:
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad()")
   if norm not in ("layer", "rms") or post_norm not in NORM_IDS:
     raise ValueError(f"{name}: norm must be 'layer' or 'rms' and post_norm one of them or None, got {norm!r} and "
                      f"{post_norm!r}")

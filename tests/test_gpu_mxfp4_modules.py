@@ -149,6 +149,57 @@ def test_input_checks_of_the_modules(cd, qt):
   assert torch.equal(y, lin.bias.expand(3, 5, 40))
 
 
+@pytest.mark.parametrize("qt", TYPES)
+def test_a_whole_transformer(cd, qt):
+  """A small FLUX-shaped model, GELU in the Linears: with the stage patch (which leaves these Linears as they are), replayed
+  from a graph, and, weight-only, against plain Linears on the dequantized weights (bf16 holds them exactly)."""
+  from cache_dit_amd import nn as cnn
+  from cache_dit_amd.testing import dit_shapes as ds
+  torch.manual_seed(5)
+  model = ds.FluxLikeTransformer(dim=256, heads=4, mlp=1024, n_double=2, n_single=2, text_dim=192, pooled_dim=96).to(BF16).cuda()
+  plain = copy.deepcopy(model)
+  cd.quantize(model, cd.QuantizeConfig(quant_type=qt))
+  converted = {n: m for n, m in model.named_modules() if isinstance(m, (cd.Mxfp4Linear, cd.Mxfp4WeightOnlyLinear))}
+  assert len(converted) >= 2 * 10 + 2 * 5 and all(m.quant_type == qt for m in converted.values())
+  for n, m in plain.named_modules():
+    if n in converted:
+      m.weight.data.copy_(cnn.dequantize_weight(converted[n]))
+  assert ds.fuse_gelu_epilogues(model) > 0
+  inputs = ds.flux_like_inputs("cuda", n_img=100, n_txt=20, text_dim=192, pooled_dim=96, seed=6)
+  with torch.no_grad():
+    out = model(**inputs)
+    out = out[0] if isinstance(out, tuple) else out
+    assert out.isfinite().all()
+    if qt == "mxfp4_weight_only":
+      want = plain(**inputs)
+      want = want[0] if isinstance(want, tuple) else want
+      # some 40 roundings to bf16 of half a step on either side, independent: 2^-9 sqrt(80), 2 % of the magnitude, 2e-4 in the cosine
+      cos = torch.nn.functional.cosine_similarity(out.double().flatten(), want.double().flatten(), dim=0)
+      assert cos >= 0.999, float(cos)
+    cd.apply_stage_patch(model)
+    patched = model(**inputs)
+    assert torch.equal(patched[0] if isinstance(patched, tuple) else patched, out)
+    cd.remove_stage_patch(model)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+      model(**inputs)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+      static = model(**inputs)
+    static = static[0] if isinstance(static, tuple) else static
+    for seed in range(3):
+      new = ds.flux_like_inputs("cuda", n_img=100, n_txt=20, text_dim=192, pooled_dim=96, seed=seed)
+      want = model(**new)
+      torch.cuda.synchronize()
+      for k in inputs:
+        inputs[k].copy_(new[k])
+      g.replay()
+      torch.cuda.synchronize()
+      assert torch.equal(static, want[0] if isinstance(want, tuple) else want), seed
+
+
 # ----------------------------------------------------------------- one after the other
 
 
