@@ -48,42 +48,32 @@ __host__ __device__ constexpr int size_of() {
   return DT == CDIT_DT_F32 ? 4 : 2;
 }
 
-// n <= 8 elements at p, the others zero. VEC: n is 0 or 8 and p is 16-byte aligned.
-template <int DT, bool VEC>
+// n <= 8 elements at p, the others zero.
+template <int DT>
 __device__ __forceinline__ void load8(const void* p, int n, float (&f)[8]) {
-  if constexpr (VEC) {
-    Mx8<DT> v = {};
-    if (n > 0) v = mx_load8<DT>(p);
-    widen8<DT>(v, f);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] = 0.0f;
-      if (i >= n) continue;
-      if constexpr (DT == CDIT_DT_F32) {
-        f[i] = static_cast<const float*>(p)[i];
-      } else if constexpr (DT == CDIT_DT_BF16) {
-        f[i] = __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
-      } else {
-        f[i] = (float)static_cast<const _Float16*>(p)[i];
-      }
+  for (int i = 0; i < 8; ++i) {
+    f[i] = 0.0f;
+    if (i >= n) continue;
+    if constexpr (DT == CDIT_DT_F32) {
+      f[i] = static_cast<const float*>(p)[i];
+    } else if constexpr (DT == CDIT_DT_BF16) {
+      f[i] = __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
+    } else {
+      f[i] = (float)static_cast<const _Float16*>(p)[i];
     }
   }
 }
-template <int DT, bool VEC>
+template <int DT>
 __device__ __forceinline__ void store8(void* p, int n, const float (&f)[8]) {
   const Mx8<DT> v = narrow8<DT>(f);
-  if constexpr (VEC) {
-    if (n > 0) mx_store8<DT>(p, v);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i >= n) continue;
-      if constexpr (DT == CDIT_DT_F32) {
-        static_cast<uint32_t*>(p)[i] = v.w[i];
-      } else {
-        static_cast<uint16_t*>(p)[i] = (uint16_t)(v.w[i / 2] >> (16 * (i & 1)));
-      }
+  for (int i = 0; i < 8; ++i) {
+    if (i >= n) continue;
+    if constexpr (DT == CDIT_DT_F32) {
+      static_cast<uint32_t*>(p)[i] = v.w[i];
+    } else {
+      static_cast<uint16_t*>(p)[i] = (uint16_t)(v.w[i / 2] >> (16 * (i & 1)));
     }
   }
 }
@@ -132,12 +122,12 @@ struct Row {
   __device__ __forceinline__ void vec(const void* p, int64_t ld, int64_t rows_per, int c, float (&f)[8]) const {
     const int64_t at = (rows_per > 0 ? row / rows_per * ld : 0) + 8 * c;
     if (a.vec_f32)
-      load8<CDIT_DT_F32, false>(static_cast<const float*>(p) + at, n_of(c), f);
+      load8<CDIT_DT_F32>(static_cast<const float*>(p) + at, n_of(c), f);
     else
-      load8<DT, false>(static_cast<const uint8_t*>(p) + at * size_of<DT>(), n_of(c), f);
+      load8<DT>(static_cast<const uint8_t*>(p) + at * size_of<DT>(), n_of(c), f);
   }
   __device__ __forceinline__ void branch(int c, float (&t)[8]) const {
-    load8<DT, false>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + 8 * c) * size_of<DT>(), n_of(c), t);
+    load8<DT>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + 8 * c) * size_of<DT>(), n_of(c), t);
   }
   // t -> post norm of t; mean and rstd of the branch's row
   __device__ __forceinline__ void post(int c, float mean, float rstd, float (&t)[8]) const {
@@ -147,7 +137,7 @@ struct Row {
     for (int i = 0; i < 8; ++i) t[i] = (t[i] - mean) * rstd * (a.post_weight ? w[i] : 1.0f);
   }
   __device__ __forceinline__ void stream(int c, float (&x)[8]) const {
-    load8<ST, false>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + 8 * c) * size_of<ST>(), n_of(c), x);
+    load8<ST>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + 8 * c) * size_of<ST>(), n_of(c), x);
   }
   // t, x -> h
   __device__ __forceinline__ void residual(int c, const float (&x)[8], float (&t)[8]) const {
@@ -177,8 +167,8 @@ struct Row {
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += f[i];
     }
-    store8<ST, false>(static_cast<uint8_t*>(a.h) + (row * a.ld_h + 8 * c) * size_of<ST>(), n, h);
-    if (a.y) store8<DT, false>(static_cast<uint8_t*>(a.y) + (row * a.ld_y + 8 * c) * size_of<DT>(), n, y);
+    store8<ST>(static_cast<uint8_t*>(a.h) + (row * a.ld_h + 8 * c) * size_of<ST>(), n, h);
+    if (a.y) store8<DT>(static_cast<uint8_t*>(a.y) + (row * a.ld_y + 8 * c) * size_of<DT>(), n, y);
     if (a.codes) {
       const Mx8<DT> v = narrow8<DT>(y);
       if (n > 0) put_codes<DT>(a, row, c, v);
@@ -218,7 +208,7 @@ __device__ __forceinline__ void statistics(const Args& a, bool layer, Sum& sum, 
   *rstd = 1.0f / __fsqrt_rn(sum(s) * inv_k + a.eps);
 }
 
-// A workgroup per row, the row read again in each pass: any K, any stride and alignment.
+// A workgroup per row, the row read again in each pass, value by value: rows of less than 8 values, or of more than 16384.
 template <int ST, int DT>
 __global__ __launch_bounds__(256) void gate_residual_norm_any(Args a) {
   __shared__ float slots[2][4];
@@ -252,11 +242,16 @@ __global__ __launch_bounds__(256) void gate_residual_norm_any(Args a) {
 // factor and an addend of the result, stay in registers until a row takes others (with one piece a lane; with two, where the
 // registers of 16 wavefronts would not hold them, each row reads them again from the caches). us, 32760 x 5120, fp32 stream,
 // one set of vectors: 604 with the vectors read for each row, 417 so (4.8 TB/s; a copy of 1 GiB runs at 5.1).
+//
+// ANY: rows of any length from 8 on, wherever they start. The last piece ends with the row and begins with values of the piece
+// before it: these count once, and are stored twice, alike. us, bf16: 8192 x 5121 83 (5120: 70), 420 with the kernel above; 20000 x 71
+// 13 and 98.
+//
 // ONCE: the 16-bit ones of x, branch and h are read and written non-temporally: they leave the caches to y or its codes, which the
 // next kernel reads. bf16, us, without and with: 8192 x 4096 with vectors per token 109 and 85 (5.5 TB/s), 4096 x 15360 126 and 114,
 // 32760 x 5120 291 and 290; below kOnceBytes, where the caches hold all of it, 2 x 4096 x 2560 36 and 42.
 constexpr int64_t kOnceBytes = (int64_t)64 << 20;
-template <int ST, int DT, int WAVES, int CH, bool ONCE>
+template <int ST, int DT, int WAVES, int CH, bool ONCE, bool ANY>
 __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, int rows_per_wg) {
   __shared__ float slots[2][WAVES];
   BlockSum<WAVES> sum{slots, 0};
@@ -265,12 +260,17 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
   const float inv_k = 1.0f / (float)a.K;
   const bool post_layer = a.post_norm == CDIT_NORM_LAYER, layer = a.norm == CDIT_NORM_LAYER;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  int col[CH];  // first column of a piece
+  int col[CH], skip[CH];  // first column of a piece, and how many of its values are the piece's before as well (ANY)
   bool in[CH];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     col[c] = 8 * ((c * WAVES + wave) * 64 + lane);
     in[c] = col[c] < a.K;
+    skip[c] = 0;
+    if (ANY && in[c]) {
+      skip[c] = max(col[c] - ((int)a.K - 8), 0);
+      col[c] -= skip[c];
+    }
   }
   auto fetch = [&](int64_t row, Mx8<DT>(&bb)[CH], Mx8<ST>(&xx)[CH]) {
 #pragma unroll
@@ -278,8 +278,8 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
       bb[c] = {};
       xx[c] = {};
       if (in[c]) {
-        bb[c] = mx_load8<DT, (ONCE && DT != CDIT_DT_F32)>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + col[c]) * size_of<DT>());
-        xx[c] = mx_load8<ST, (ONCE && ST != CDIT_DT_F32)>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + col[c]) * size_of<ST>());
+        bb[c] = mx_load8<DT, (ONCE && DT != CDIT_DT_F32), ANY>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + col[c]) * size_of<DT>());
+        xx[c] = mx_load8<ST, (ONCE && ST != CDIT_DT_F32), ANY>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + col[c]) * size_of<ST>());
       }
     }
   };
@@ -289,10 +289,15 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
   float vg[KEPT][8], vm[KEPT][8], vs[KEPT][8];
   int64_t at_gate = -1, at_shift = -1, at_scale = -1;
   auto vector = [&](const void* p, int64_t at, int c, float(&f)[8]) {
-    if (a.vec_f32)
-      load8<CDIT_DT_F32, true>(static_cast<const float*>(p) + at + col[c], in[c] ? 8 : 0, f);
-    else
-      load8<DT, true>(static_cast<const uint8_t*>(p) + (at + col[c]) * size_of<DT>(), in[c] ? 8 : 0, f);
+    if (a.vec_f32) {
+      Mx8<CDIT_DT_F32> v = {};
+      if (in[c]) v = mx_load8<CDIT_DT_F32, false, ANY>(static_cast<const float*>(p) + at + col[c]);
+      widen8<CDIT_DT_F32>(v, f);
+    } else {
+      Mx8<DT> v = {};
+      if (in[c]) v = mx_load8<DT, false, ANY>(static_cast<const uint8_t*>(p) + (at + col[c]) * size_of<DT>());
+      widen8<DT>(v, f);
+    }
   };
   auto branch_factor = [&](int c, float(&f)[8]) {
     float w[8];
@@ -345,7 +350,7 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += f[c][i];  // (pieces behind the row are zeros)
+        for (int i = 0; i < 8; ++i) s += ANY && i < skip[c] ? 0.0f : f[c][i];  // (pieces behind the row are zeros)
       *mean = sum(s) * inv_k;
       s = 0.0f;
     }
@@ -353,7 +358,7 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float d = in[c] ? f[c][i] - *mean : 0.0f;
+        const float d = in[c] && !(ANY && i < skip[c]) ? f[c][i] - *mean : 0.0f;
         s = __fmaf_rn(d, d, s);
       }
     *rstd = 1.0f / __fsqrt_rn(sum(s) * inv_k + a.eps);
@@ -388,10 +393,10 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         y[i] = __fmaf_rn((h[c][i] - mean) * rstd, KEEP ? vm[KEEP ? c : 0][i] : m[i], KEEP ? vs[KEEP ? c : 0][i] : s[i]);
-      mx_store8<ST, (ONCE && ST != CDIT_DT_F32)>(static_cast<uint8_t*>(a.h) + (row * a.ld_h + col[c]) * size_of<ST>(),
+      mx_store8<ST, (ONCE && ST != CDIT_DT_F32), ANY>(static_cast<uint8_t*>(a.h) + (row * a.ld_h + col[c]) * size_of<ST>(),
                                                  narrow8<ST>(h[c]));
       const Mx8<DT> v = narrow8<DT>(y);
-      if (a.y) mx_store8<DT>(static_cast<uint8_t*>(a.y) + (row * a.ld_y + col[c]) * size_of<DT>(), v);
+      if (a.y) mx_store8<DT, false, ANY>(static_cast<uint8_t*>(a.y) + (row * a.ld_y + col[c]) * size_of<DT>(), v);
       if (a.codes) put_codes<DT>(a, row, col[c] / 8, v);
     }
   };
@@ -404,39 +409,52 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
   }
 }
 
+// Whether every piece of 8 columns starts on 16 bytes.
 template <int ST, int DT>
-bool rows_fit(const Args& a) {
+bool rows_aligned(const Args& a) {
   constexpr int SS = size_of<ST>(), DS = size_of<DT>();
   auto rows = [](const void* p, int64_t ld, int size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0;
   };
   const int vs = a.vec_f32 ? 4 : DS;
   auto vec = [&](const void* p, int64_t ld) { return !p || rows(p, ld, vs); };
-  return a.K % 8 == 0 && a.K <= 16384 && rows(a.x, a.ld_x, SS) && rows(a.h, a.ld_h, SS) && rows(a.branch, a.ld_branch, DS) &&
+  return a.K % 8 == 0 && rows(a.x, a.ld_x, SS) && rows(a.h, a.ld_h, SS) && rows(a.branch, a.ld_branch, DS) &&
          (!a.y || rows(a.y, a.ld_y, DS)) && vec(a.gate, a.ld_gate) && vec(a.shift, a.ld_shift) && vec(a.scale, a.ld_scale) &&
          vec(a.norm_weight, 0) && vec(a.post_weight, 0);
 }
 
 template <int ST, int DT>
 int launch_types(const Args& a, hipStream_t stream) {
-  if (rows_fit<ST, DT>(a)) {
+  if (a.K >= 8 && a.K <= 16384) {
     const int cus = cu_count();
     if (cus <= 0) {
       set_error("cannot query the CU count of the current device");
       return CDIT_EHIP;
     }
-    const int pieces = (int)(a.K / 8);
-    const bool once = 2 * a.M * a.K >= kOnceBytes;
-#define CDIT_NORM_CASE(W, CH)                                                                                         \
-  if (pieces <= 64 * W * CH) {                                                                                        \
-    const int64_t target = (int64_t)cus * std::max(1, 24 / W);                                                        \
-    const int per = (int)std::min<int64_t>((a.M + target - 1) / target, 1 << 20);                                     \
-    const dim3 grid((unsigned)((a.M + per - 1) / per));                                                               \
-    if (once)                                                                                                         \
-      hipLaunchKernelGGL((gate_residual_norm_rows<ST, DT, W, CH, DT != CDIT_DT_F32>), grid, dim3(64 * W), 0, stream, a, per); \
-    else                                                                                                              \
-      hipLaunchKernelGGL((gate_residual_norm_rows<ST, DT, W, CH, false>), grid, dim3(64 * W), 0, stream, a, per);     \
-    return 0;                                                                                                         \
+    const int pieces = (int)((a.K + 7) / 8);
+    const bool once = DT != CDIT_DT_F32 && 2 * a.M * a.K >= kOnceBytes, aligned = rows_aligned<ST, DT>(a);
+    auto launch = [&](auto kernel, int waves) {
+      const int64_t target = (int64_t)cus * std::max(1, 24 / waves);
+      const int per = (int)std::min<int64_t>((a.M + target - 1) / target, 1 << 20);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((a.M + per - 1) / per)), dim3(64 * waves), 0, stream, a, per);
+      return 0;
+    };
+    if (!aligned) {
+#define CDIT_NORM_CASE(W, CH) \
+  if (pieces <= 64 * W * CH) return launch(gate_residual_norm_rows<ST, DT, W, CH, false, true>, W);
+      CDIT_NORM_CASE(1, 1)
+      CDIT_NORM_CASE(2, 1)
+      CDIT_NORM_CASE(4, 1)
+      CDIT_NORM_CASE(8, 1)
+      CDIT_NORM_CASE(12, 1)
+      CDIT_NORM_CASE(16, 1)
+      CDIT_NORM_CASE(16, 2)
+#undef CDIT_NORM_CASE
+    }
+#define CDIT_NORM_CASE(W, CH)                                                                              \
+  if (pieces <= 64 * W * CH) {                                                                             \
+    if (once) return launch(gate_residual_norm_rows<ST, DT, W, CH, DT != CDIT_DT_F32, false>, W);          \
+    return launch(gate_residual_norm_rows<ST, DT, W, CH, false, false>, W);                                \
   }
     CDIT_NORM_CASE(1, 1)
     CDIT_NORM_CASE(2, 1)

@@ -46,15 +46,25 @@ template <int DT>
 struct Mx8 {
   uint32_t w[DT == CDIT_DT_F32 ? 8 : 4];
 };
-template <int DT, bool ONCE = false>  // ONCE: non-temporal, read by nobody else soon
+// At 16 bytes, or (ANY) wherever an element may be: the hardware takes such accesses.
+template <bool ANY>
+struct MxPart {
+  typedef mx_v4u type;
+};
+template <>
+struct MxPart<true> {
+  typedef mx_v4u type __attribute__((aligned(2)));
+};
+template <int DT, bool ONCE = false, bool ANY = false>  // ONCE: non-temporal, read by nobody else soon
 __device__ __forceinline__ Mx8<DT> mx_load8(const void* p) {
+  typedef typename MxPart<ANY>::type Part;
   Mx8<DT> v;
-  auto load = [](const mx_v4u* q) { return ONCE ? __builtin_nontemporal_load(q) : *q; };
-  const mx_v4u a = load(reinterpret_cast<const mx_v4u*>(p));
+  auto load = [](const Part* q) -> mx_v4u { return ONCE ? __builtin_nontemporal_load(q) : *q; };
+  const mx_v4u a = load(static_cast<const Part*>(p));
 #pragma unroll
   for (int i = 0; i < 4; ++i) v.w[i] = a[i];
   if constexpr (DT == CDIT_DT_F32) {
-    const mx_v4u b = load(reinterpret_cast<const mx_v4u*>(p) + 1);
+    const mx_v4u b = load(static_cast<const Part*>(p) + 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v.w[4 + i] = b[i];
   }
@@ -137,16 +147,17 @@ __device__ __forceinline__ Mx8<DT> mx_values8(uint32_t c, int e) {
   }
   return v;
 }
-template <int DT, bool ONCE = false>
+template <int DT, bool ONCE = false, bool ANY = false>
 __device__ __forceinline__ void mx_store8(void* p, const Mx8<DT>& v) {
-  auto store = [](mx_v4u d, mx_v4u* q) {
+  typedef typename MxPart<ANY>::type Part;
+  auto store = [](mx_v4u d, Part* q) {
     if (ONCE)
       __builtin_nontemporal_store(d, q);
     else
       *q = d;
   };
-  store(mx_v4u{v.w[0], v.w[1], v.w[2], v.w[3]}, reinterpret_cast<mx_v4u*>(p));
-  if constexpr (DT == CDIT_DT_F32) store(mx_v4u{v.w[4], v.w[5], v.w[6], v.w[7]}, reinterpret_cast<mx_v4u*>(p) + 1);
+  store(mx_v4u{v.w[0], v.w[1], v.w[2], v.w[3]}, static_cast<Part*>(p));
+  if constexpr (DT == CDIT_DT_F32) store(mx_v4u{v.w[4], v.w[5], v.w[6], v.w[7]}, static_cast<Part*>(p) + 1);
 }
 
 // Eight codes as bf16, times their scale.

@@ -93,6 +93,14 @@ def test_widths(ops, K, norm):
   run_case(ops, (2, 3), K, BF16, BF16, norm, "rms-w" if K % 3 else None, "batch", eps=1e-6 if K > 1 else 1e-2)
 
 
+@pytest.mark.parametrize("K", [8, 9, 15, 17, 71, 505, 519, 1025, 2047, 4097, 6151, 8193, 15001, 16383, 16385])
+@pytest.mark.parametrize("dtype,stream", TYPES)
+def test_rows_of_any_length(ops, K, dtype, stream):
+  """Pieces of 8 that end with the row; every lane's, wavefront's and register's edge."""
+  run_case(ops, (2, 3), K, dtype, stream, "layer", "layer", "batch", seed=K)
+  run_case(ops, (1, 4), K, dtype, stream, "rms", None, "token", seed=K + 1)
+
+
 @pytest.mark.parametrize("shape", [(1, 1), (1, ), (3, ), (1, 700), (5, 401), (2, 3, 4)])
 def test_rows(ops, shape):
   run_case(ops, shape, 1280, BF16, F32, "layer", "rms-w", "batch" if len(shape) > 1 else "one")
