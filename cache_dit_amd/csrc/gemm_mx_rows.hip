@@ -1,6 +1,6 @@
-// The 4-bit Linears for up to 16 rows (single tokens, conditioning vectors): a stream of weights.
+// The 4-bit Linears for few rows (single tokens, conditioning vectors): a stream of weights.
 //
-// A workgroup takes G times 16 output columns. The activation goes to LDS first (in pieces of K where it is long), and is
+// A workgroup takes 16 rows (or the less there are) and G times 16 output columns. The activation goes to LDS first (in pieces of K where it is long), and is
 // quantized on the way where the caller has it in bf16. K is split between the W wavefronts in items of 512; a wavefront reads an
 // item's weights straight from memory (every byte is used once, the next item's loads are under way meanwhile) and multiplies
 // them with the activation's rows on the matrix core, and the W partial sums of 16 x 16 outputs meet in LDS. Bound by HBM, and
@@ -21,6 +21,7 @@ namespace {
 
 // Weight-only: bf16 activation. Codes: an activation in MXFP4. Quantize: a bf16 activation, quantized here.
 enum Mode { kWeightOnly, kCodes, kQuantize };
+constexpr int kMostRows = 16;         // of a workgroup
 constexpr int kItem = 512;            // along K
 constexpr int kMostWaves = 8;
 constexpr int kMostLds = 64 * 1024;   // of activation and scales: two workgroups fit a CU
@@ -33,6 +34,13 @@ __host__ __device__ constexpr int scale_pitch(int items) { return items * 16 + 4
 template <int MODE, int OUT>
 __global__ __launch_bounds__(64 * kMostWaves) void gemm_mx_rows(Mx4Gemm g, int G, int chunk_items) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  {  // this workgroup's rows
+    const int64_t m0 = kMostRows * (int64_t)blockIdx.y;
+    g.a += m0 * g.lda * (MODE == kCodes ? 1 : 2);
+    if (MODE == kCodes) g.a_scale += m0 * g.ldas;
+    g.out = static_cast<uint8_t*>(g.out) + m0 * g.ldo * (OUT == CDIT_DT_F32 ? 4 : 2);
+    g.M = min(g.M - (int)m0, kMostRows);
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, kg = lane >> 4;
   const int KB = g.K / kMxBlock, S = (g.K + 127) / 128 * 4, items = (g.K + kItem - 1) / kItem;
@@ -210,13 +218,14 @@ int launch_rows(const Mx4Gemm& g, hipStream_t stream) {
   // 12.8 us with 5 or 8, 15.6 with 10; K 16384 33.2 with 8, 41.1 with 16.
   const int G = groups > 2 * cus ? 2 : 1;
   // as many items of the activation and of scales as fit; even shares of them for the wavefronts
-  auto bytes = [&](int n) { return g.M * (row_pitch(MODE, n) + scale_pitch(n)) + 16 * G * scale_pitch(n); };
+  const int M = std::min(g.M, kMostRows), blocks = (g.M + kMostRows - 1) / kMostRows;
+  auto bytes = [&](int n) { return M * (row_pitch(MODE, n) + scale_pitch(n)) + 16 * G * scale_pitch(n); };
   int chunk = items;
   while (chunk > 1 && bytes(chunk) > kMostLds) --chunk;
   const int per = (chunk + kMostWaves - 1) / kMostWaves, waves = (chunk + per - 1) / per;
   const int lds = G * waves * 1024 + bytes(chunk);
   if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&gemm_mx_rows<MODE, OUT>), 160 * 1024, lds_allowed)) return rc;
-  hipLaunchKernelGGL((gemm_mx_rows<MODE, OUT>), dim3((unsigned)((groups + G - 1) / G)), dim3(64 * waves), lds, stream, g, G,
+  hipLaunchKernelGGL((gemm_mx_rows<MODE, OUT>), dim3((unsigned)((groups + G - 1) / G), (unsigned)blocks), dim3(64 * waves), lds, stream, g, G,
                      chunk);
   return 0;
 }
@@ -231,15 +240,23 @@ int launch_rows(const Mx4Gemm& g, hipStream_t stream) {
 
 }  // namespace
 
-// Whether this is the kernel for so many rows and columns, and not a tile. Every workgroup handles the whole activation, so its
+// Whether this is the kernel for up to 16 rows and so many columns, and not a tile. Every workgroup handles the whole activation, so its
 // time grows with rows times columns; us, this kernel and the best tile (w4a4 with its quantizer), M x N x K, weights from HBM:
 // w4a4 4 x 13824 x 5120 14.9 and 18.1, 8: 17.1 and 18.5, 16: 21.2 and 18.2; 16 x 5120 x 5120 14.0 and 14.8; 16 x 30720 x 5120 38.8
 // and 25.5. Weight-only 8 x 13824 x 5120 17.9 and 24.4, 16: 23.7 and 25.1; 16 x 30720 x 5120 45.9 and 32.4.
 bool mx_rows_fit(bool weight_only, int64_t M, int64_t N, int64_t ldb) {
-  return mx_rows_can(M, ldb) && M * ((N + 15) / 16) < (weight_only ? 20000 : 10000);
+  return mx_rows_can(M, ldb) && M <= 16 && M * ((N + 15) / 16) < (weight_only ? 20000 : 10000);
 }
-// Whether it can take them: 16 rows of the activation, and of the weight 16 within 32-bit offsets.
-bool mx_rows_can(int64_t M, int64_t ldb) { return M >= 1 && M <= 16 && ldb < (int64_t)1 << 27; }
+// Its time for more than 16 rows, ns, next to the tiles': a workgroup per 16 x 16 outputs reads little for each of its steps along K
+// and so is done first where the tiles leave CUs idle. us, this kernel and the best tile, M x N x K: w4a4 294 x 16 x 9248 8.9 and
+// 13.8, 502 x 128 x 5856 7.0 and 10.0, 32 x 1024 x 15360 14.8 and 20.4, 17 x 5120 x 5120 10.5 and 9.4; w4a16 19.6 and 24.1, 16.8
+// and 21.0, 30.0 and 53.2, 18.4 and 19.1.
+int64_t mx_rows_ns(bool weight_only, int64_t M, int64_t N, int64_t K) {
+  const int64_t items = (K + kItem - 1) / kItem, blocks = (M + kMostRows - 1) / kMostRows * ((N + 15) / 16);
+  return 4000 + (weight_only ? 870 : 270) * items + std::max<int64_t>(blocks - 256, 0) * items * (weight_only ? 240 : 115) / 100;
+}
+// Whether it can take them: 16 rows of the weight within 32-bit offsets.
+bool mx_rows_can(int64_t M, int64_t ldb) { return M >= 1 && M <= 65535 * kMostRows && ldb < (int64_t)1 << 27; }
 
 int launch_gemm_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream) { return launch_rows<kCodes>(g, stream); }
 int launch_linear_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream) { return launch_rows<kQuantize, CDIT_DT_BF16>(g, stream); }

@@ -400,7 +400,7 @@ static const MxTime kTimes[] = {
 int choose_gemm_mxfp4(const Mx4Gemm& g) {
   if (mx_rows_fit(false, g.M, g.N, g.ldb)) return kMxRows;
   const int cus = cu_count();
-  return tiles_fit(g, 1) ? fastest_tile(kTimes, sizeof(kTimes) / sizeof(kTimes[0]), g, cus > 0 ? cus : 256) : 0;
+  return tiles_fit(g, 1) ? fastest_tile(kTimes, sizeof(kTimes) / sizeof(kTimes[0]), false, g, cus > 0 ? cus : 256) : 0;
 }
 
 int launch_gemm_mxfp4(const Mx4Gemm& g, int variant, hipStream_t stream) {

@@ -17,12 +17,16 @@ namespace {
 struct MxTime {
   int variant, bm, bn, start, tile, lone, step;
 };
-// The tile with the least time. Tiles beyond whole rounds of the CUs count half a round and half their share of one: fewer CUs
+// The tile with the least time, or the kernel for few rows where it takes less. Tiles beyond whole rounds of the CUs count half a round and half their share of one: fewer CUs
 // share the memory and the power then.
-inline int fastest_tile(const MxTime* t, int count, const Mx4Gemm& g, int cus) {
+inline int fastest_tile(const MxTime* t, int count, bool weight_only, const Mx4Gemm& g, int cus) {
   const int64_t steps = (g.K + 255) / 256;
   int best = -1;
   int64_t best_ns = 0;
+  if (mx_rows_can(g.M, g.ldb) && g.M > 16) {
+    best = kMxRows;
+    best_ns = mx_rows_ns(weight_only, g.M, g.N, g.K);
+  }
   for (int i = 0; i < count; ++i) {
     const int64_t tiles = (int64_t)((g.M + t[i].bm - 1) / t[i].bm) * ((g.N + t[i].bn - 1) / t[i].bn);
     const int64_t permille = tiles <= cus ? 1000 : rounds_permille(tiles, cus, 500, 500);

@@ -394,8 +394,8 @@ int cdit_mxfp4_gemm(const void* a_codes, const void* a_scales, const void* b_cod
 
 /*
  * One Linear forward in that mode: cdit_mxfp4_quant of x (bf16 [M,K], ld_x) into the caller's workspaces (codes_ws
- * M * K/2 bytes, scales_ws M * 4 ceil(K/128) bytes, both on 16 bytes), then cdit_mxfp4_gemm; out and bias bf16. For few
- * rows (up to 16, as the columns allow) one kernel quantizes the rows itself; the workspaces are then not written.
+ * M * K/2 bytes, scales_ws M * 4 ceil(K/128) bytes, both on 16 bytes), then cdit_mxfp4_gemm; out and bias bf16. For up
+ * to 16 rows (as the columns allow) one kernel quantizes the rows itself; the workspaces are then not written.
  */
 int cdit_mxfp4_linear(const void* x_bf16, const void* w_codes, const void* w_scales, const void* bias_bf16, void* out,
                       void* codes_ws, void* scales_ws, int64_t M, int64_t N, int64_t K, int64_t ld_x, int64_t ldw,

@@ -404,6 +404,19 @@ def test_few_rows(cd, variant, M, N, K):
     check_product(cd.ops.w4a16_mm(x, codes, scales, bias), x, codes, scales, bias, "mxfp4_weight_only")
 
 
+@pytest.mark.parametrize("M,N,K", [(17, 100, 5120), (33, 16, 9248), (48, 40, 20000 // 32 * 32), (300, 130, 544), (500, 33, 2048)])
+def test_few_columns(cd, variant, M, N, K):
+  """More than 16 rows of the kernel for few, where it is chosen and where it is not."""
+  x, w, bias = rand(M, K, seed=M), rand(N, K, seed=N, std=0.05), rand(N, seed=K, std=0.1)
+  codes, scales = cd.mxfp4_quant(w)
+  for v in (-1, 100):
+    variant(v)
+    check_product(cd.ops.mxfp4_linear(x, codes, scales, bias), x, codes, scales, bias, "mxfp4")
+    check_product(cd.ops.w4a16_mm(x, codes, scales, bias, 1), x, codes, scales, bias, "mxfp4_weight_only", gelu=True)
+    got = cd.mxfp4_mm(*cd.mxfp4_quant(x), codes, scales, torch.float32, bias)
+    check_product(got, x, codes, scales, bias, "mxfp4")
+
+
 # -------------------------------------------------------------------- beyond 32 bits
 
 
@@ -490,7 +503,7 @@ def rest_is_untouched(m, view):
   assert (m == 0x5a).all()
 
 
-@pytest.mark.parametrize("v", [-1, 0, 1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("v", [-1, 0, 1, 2, 3, 4, 5, 6, 7, 8, 100])
 @pytest.mark.parametrize("M,N,K", [(1, 77, 96), (13, 33, 544), (70, 131, 160), (300, 260, 512)])
 def test_nothing_but_the_outputs_is_written(cd, variant, v, M, N, K):
   """Outputs, codes, scales and workspaces with rows further apart than they are long, in memory that is looked over."""
