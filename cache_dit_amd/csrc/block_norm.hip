@@ -278,8 +278,10 @@ __global__ __launch_bounds__(64 * WAVES) void gate_residual_norm_rows(Args a, in
       bb[c] = {};
       xx[c] = {};
       if (in[c]) {
-        bb[c] = mx_load8<DT, (ONCE && DT != CDIT_DT_F32), ANY>(static_cast<const uint8_t*>(a.branch) + (row * a.ld_branch + col[c]) * size_of<DT>());
-        xx[c] = mx_load8<ST, (ONCE && ST != CDIT_DT_F32), ANY>(static_cast<const uint8_t*>(a.x) + (row * a.ld_x + col[c]) * size_of<ST>());
+        bb[c] = mx_load8<DT, (ONCE && DT != CDIT_DT_F32), ANY>(static_cast<const uint8_t*>(a.branch) +
+                                                               (row * a.ld_branch + col[c]) * size_of<DT>());
+        xx[c] = mx_load8<ST, (ONCE && ST != CDIT_DT_F32), ANY>(static_cast<const uint8_t*>(a.x) +
+                                                               (row * a.ld_x + col[c]) * size_of<ST>());
       }
     }
   };

@@ -1,7 +1,7 @@
 // The 4-bit Linears for few rows (single tokens, conditioning vectors): a stream of weights.
 //
-// A workgroup takes 16 rows (or the less there are) and G times 16 output columns. The activation goes to LDS first (in pieces of K where it is long), and is
-// quantized on the way where the caller has it in bf16. K is split between the W wavefronts in items of 512; a wavefront reads an
+// A workgroup takes 16 rows (or the less there are) and G times 16 output columns. The activation goes to LDS first (in pieces of K
+// where it is long), and is quantized on the way where the caller has it in bf16. K is split between the W wavefronts in items of 512; a wavefront reads an
 // item's weights straight from memory (every byte is used once, the next item's loads are under way meanwhile) and multiplies
 // them with the activation's rows on the matrix core, and the W partial sums of 16 x 16 outputs meet in LDS. Bound by HBM, and
 // by latency where N is small: 1 x 30720 x 5120 (M x N x K) 17.9 us for 84 MB, where a kernel that only reads them takes 14.8; 1 x
@@ -240,8 +240,8 @@ int launch_rows(const Mx4Gemm& g, hipStream_t stream) {
 
 }  // namespace
 
-// Whether this is the kernel for up to 16 rows and so many columns, and not a tile. Every workgroup handles the whole activation, so its
-// time grows with rows times columns; us, this kernel and the best tile (w4a4 with its quantizer), M x N x K, weights from HBM:
+// Whether this is the kernel for up to 16 rows and so many columns, and not a tile. Every workgroup handles the whole activation, so
+// its time grows with rows times columns; us, this kernel and the best tile (w4a4 with its quantizer), M x N x K, weights from HBM:
 // w4a4 4 x 13824 x 5120 14.9 and 18.1, 8: 17.1 and 18.5, 16: 21.2 and 18.2; 16 x 5120 x 5120 14.0 and 14.8; 16 x 30720 x 5120 38.8
 // and 25.5. Weight-only 8 x 13824 x 5120 17.9 and 24.4, 16: 23.7 and 25.1; 16 x 30720 x 5120 45.9 and 32.4.
 bool mx_rows_fit(bool weight_only, int64_t M, int64_t N, int64_t ldb) {

@@ -17,8 +17,8 @@ namespace {
 struct MxTime {
   int variant, bm, bn, start, tile, lone, step;
 };
-// The tile with the least time, or the kernel for few rows where it takes less. Tiles beyond whole rounds of the CUs count half a round and half their share of one: fewer CUs
-// share the memory and the power then.
+// The tile with the least time, or the kernel for few rows where it takes less. Tiles beyond whole rounds of the CUs count half a
+// round and half their share of one: fewer CUs share the memory and the power then.
 inline int fastest_tile(const MxTime* t, int count, bool weight_only, const Mx4Gemm& g, int cus) {
   const int64_t steps = (g.K + 255) / 256;
   int best = -1;
