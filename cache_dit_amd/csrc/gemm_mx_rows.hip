@@ -1,8 +1,8 @@
 // The 4-bit Linears for few rows (single tokens, conditioning vectors): a stream of weights.
 //
 // A workgroup takes 16 rows (or the less there are) and G times 16 output columns. The activation goes to LDS first (in pieces of K
-// where it is long), and is quantized on the way where the caller has it in bf16. K is split between the W wavefronts in items of 512; a wavefront reads an
-// item's weights straight from memory (every byte is used once, the next item's loads are under way meanwhile) and multiplies
+// where it is long), and is quantized on the way where the caller has it in bf16. K is split between the W wavefronts in items of
+// 512; a wavefront reads an item's weights straight from memory (every byte is used once, the next item's loads are under way meanwhile) and multiplies
 // them with the activation's rows on the matrix core, and the W partial sums of 16 x 16 outputs meet in LDS. Bound by HBM, and
 // by latency where N is small: 1 x 30720 x 5120 (M x N x K) 17.9 us for 84 MB, where a kernel that only reads them takes 14.8; 1 x
 // 13824 x 5120 10.8 with the weight in the caches as far as it fits, 12.8 from HBM (8.2 to only read it).
