@@ -14,6 +14,7 @@
 #include <algorithm>
 
 #include "gemm_common.h"
+#include "mx_rows_plan.h"
 #include "mxfp4_device.h"
 
 namespace cdit {
@@ -21,18 +22,10 @@ namespace {
 
 // Weight-only: bf16 activation. Codes: an activation in MXFP4. Quantize: a bf16 activation, quantized here.
 enum Mode { kWeightOnly, kCodes, kQuantize };
-constexpr int kMostRows = 16;         // of a workgroup
-constexpr int kItem = 512;            // along K
-constexpr int kMostWaves = 8;
-constexpr int kMostLds = 64 * 1024;   // of activation and scales: two workgroups fit a CU
-
-// Bytes of a row of the activation in LDS for `items` items, and of a row of scales. 16 (4) more than a multiple of 256 (16): the
-// 16 rows a pass reads start in different banks.
-__host__ __device__ constexpr int row_pitch(int mode, int items) { return items * (mode == kWeightOnly ? 1024 : 256) + 16; }
-__host__ __device__ constexpr int scale_pitch(int items) { return items * 16 + 4; }
+constexpr int kMostRows = kMxRowsMost, kItem = kMxRowsItem;
 
 template <int MODE, int OUT>
-__global__ __launch_bounds__(64 * kMostWaves) void gemm_mx_rows(Mx4Gemm g, int G, int chunk_items) {
+__global__ __launch_bounds__(64 * kMxRowsWaves) void gemm_mx_rows(Mx4Gemm g, int G, int chunk_items) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   {  // this workgroup's rows
     const int64_t m0 = kMostRows * (int64_t)blockIdx.y;
@@ -44,10 +37,10 @@ __global__ __launch_bounds__(64 * kMostWaves) void gemm_mx_rows(Mx4Gemm g, int G
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, kg = lane >> 4;
   const int KB = g.K / kMxBlock, S = (g.K + 127) / 128 * 4, items = (g.K + kItem - 1) / kItem;
-  const int pitch = row_pitch(MODE, chunk_items), spitch = MODE == kWeightOnly ? 0 : scale_pitch(chunk_items);
+  const int pitch = mx_row_pitch(MODE == kWeightOnly, chunk_items), spitch = MODE == kWeightOnly ? 0 : mx_scale_pitch(chunk_items);
   float* const part = reinterpret_cast<float*>(smem);  // [G][waves][256]
   uint8_t* const wscale = smem + G * waves * 1024;  // [16 G][wpitch]
-  const int wpitch = scale_pitch(chunk_items);
+  const int wpitch = mx_scale_pitch(chunk_items);
   uint8_t* const xs = wscale + 16 * G * wpitch;
   uint8_t* const xe = xs + g.M * pitch;
   const int m = min(r, g.M - 1);  // (rows that do not exist repeat the last: their results are not stored)
@@ -212,21 +205,11 @@ int launch_rows(const Mx4Gemm& g, hipStream_t stream) {
     set_error("cannot query the CU count of the current device");
     return CDIT_EHIP;
   }
-  const int items = std::max(1, (g.K + kItem - 1) / kItem), groups = (g.N + 15) / 16;
-  // Two groups of columns a workgroup where there are more than two for each CU: 30720 columns, K 5120, one row 23.1 us with one,
-  // 21.5 with two, 23.9 with four (5 wavefronts; 10 are slower throughout). 8 wavefronts at most: 13824 columns, K 5120
-  // 12.8 us with 5 or 8, 15.6 with 10; K 16384 33.2 with 8, 41.1 with 16.
-  const int G = groups > 2 * cus ? 2 : 1;
-  // as many items of the activation and of scales as fit; even shares of them for the wavefronts
-  const int M = std::min(g.M, kMostRows), blocks = (g.M + kMostRows - 1) / kMostRows;
-  auto bytes = [&](int n) { return M * (row_pitch(MODE, n) + scale_pitch(n)) + 16 * G * scale_pitch(n); };
-  int chunk = items;
-  while (chunk > 1 && bytes(chunk) > kMostLds) --chunk;
-  const int per = (chunk + kMostWaves - 1) / kMostWaves, waves = (chunk + per - 1) / per;
-  const int lds = G * waves * 1024 + bytes(chunk);
+  const MxRowsPlan p = mx_rows_plan(MODE == kWeightOnly, g.M, g.N, g.K, cus);
+  const int groups = (g.N + 15) / 16, blocks = (g.M + kMostRows - 1) / kMostRows;
   if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&gemm_mx_rows<MODE, OUT>), 160 * 1024, lds_allowed)) return rc;
-  hipLaunchKernelGGL((gemm_mx_rows<MODE, OUT>), dim3((unsigned)((groups + G - 1) / G), (unsigned)blocks), dim3(64 * waves), lds, stream, g, G,
-                     chunk);
+  hipLaunchKernelGGL((gemm_mx_rows<MODE, OUT>), dim3((unsigned)((groups + p.groups - 1) / p.groups), (unsigned)blocks),
+                     dim3(64 * p.waves), p.lds, stream, g, p.groups, p.chunk);
   return 0;
 }
 template <int MODE>
