@@ -148,7 +148,7 @@ int choose_gemm_w4a16(const Mx4Gemm& g);
 // Few rows (gemm_mx_rows.hip). The Linear: g.a is the bf16 activation, g.lda in elements; the kernel quantizes it.
 bool mx_rows_fit(bool weight_only, int64_t M, int64_t N, int64_t ldb);
 bool mx_rows_can(int64_t M, int64_t ldb);
-int64_t mx_rows_ns(bool weight_only, int64_t M, int64_t N, int64_t K);
+int64_t mx_rows_ns(bool weight_only, int64_t M, int64_t N, int64_t K, int64_t cus);
 int launch_gemm_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream);
 int launch_linear_mxfp4_rows(const Mx4Gemm& g, hipStream_t stream);
 int launch_gemm_w4a16_rows(const Mx4Gemm& g, hipStream_t stream);

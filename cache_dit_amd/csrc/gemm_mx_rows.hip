@@ -234,9 +234,9 @@ bool mx_rows_fit(bool weight_only, int64_t M, int64_t N, int64_t ldb) {
 // and so is done first where the tiles leave CUs idle. us, this kernel and the best tile, M x N x K: w4a4 294 x 16 x 9248 8.9 and
 // 13.8, 502 x 128 x 5856 7.0 and 10.0, 32 x 1024 x 15360 14.8 and 20.4, 17 x 5120 x 5120 10.5 and 9.4; w4a16 19.6 and 24.1, 16.8
 // and 21.0, 30.0 and 53.2, 18.4 and 19.1.
-int64_t mx_rows_ns(bool weight_only, int64_t M, int64_t N, int64_t K) {
+int64_t mx_rows_ns(bool weight_only, int64_t M, int64_t N, int64_t K, int64_t cus) {
   const int64_t items = (K + kItem - 1) / kItem, blocks = (M + kMostRows - 1) / kMostRows * ((N + 15) / 16);
-  return 4000 + (weight_only ? 870 : 270) * items + std::max<int64_t>(blocks - 256, 0) * items * (weight_only ? 240 : 115) / 100;
+  return 4000 + (weight_only ? 870 : 270) * items + std::max<int64_t>(blocks - cus, 0) * items * (weight_only ? 240 : 115) / 100;
 }
 // Whether it can take them: 16 rows of the weight within 32-bit offsets.
 bool mx_rows_can(int64_t M, int64_t ldb) { return M >= 1 && M <= 65535 * kMostRows && ldb < (int64_t)1 << 27; }

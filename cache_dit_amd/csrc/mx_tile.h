@@ -25,7 +25,7 @@ inline int fastest_tile(const MxTime* t, int count, bool weight_only, const Mx4G
   int64_t best_ns = 0;
   if (mx_rows_can(g.M, g.ldb) && g.M > 16) {
     best = kMxRows;
-    best_ns = mx_rows_ns(weight_only, g.M, g.N, g.K);
+    best_ns = mx_rows_ns(weight_only, g.M, g.N, g.K, cus);
   }
   for (int i = 0; i < count; ++i) {
     const int64_t tiles = (int64_t)((g.M + t[i].bm - 1) / t[i].bm) * ((g.N + t[i].bn - 1) / t[i].bn);

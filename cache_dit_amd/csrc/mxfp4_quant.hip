@@ -24,10 +24,10 @@ struct Runs {
   }
 };
 // 2048 pieces a workgroup, eight a thread, where there are many; one a thread where that leaves CUs idle.
-Runs runs_of(int64_t M, int64_t K) {
+Runs runs_of(int64_t M, int64_t K, int cus) {
   const int per_row = (int)(K / 8);
   const int rows = per_row >= 1024 ? 1 : 2048 / per_row;
-  const int64_t pieces = M * per_row, wanted = 4 * 256;
+  const int64_t pieces = M * per_row, wanted = 4 * (int64_t)cus;
   const int span = (int)std::min<int64_t>(2048, std::max<int64_t>(kThreads, (pieces / wanted + kThreads - 1) / kThreads * kThreads));
   return {rows, per_row, span, (uint32_t)(((uint64_t(1) << 32) + per_row - 1) / per_row)};
 }
@@ -113,7 +113,12 @@ __global__ __launch_bounds__(kThreads) void mxfp4_dequant_rows(const uint8_t* __
 
 int launch_mxfp4_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ld_x, void* codes, int64_t ld_codes,
                        void* scales, int64_t ld_scales, hipStream_t stream) {
-  const Runs r = runs_of(M, K);
+  const int cus = cu_count();
+  if (cus <= 0) {
+    set_error("cannot query the CU count of the current device");
+    return CDIT_EHIP;
+  }
+  const Runs r = runs_of(M, K, cus);
   const dim3 grid = r.grid(M);
   const bool once = 2 * M * K > kOnceBytes;
 #define CDIT_MXQ(DT, ONCE)                                                                                          \
@@ -135,7 +140,12 @@ int launch_mxfp4_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t l
 
 int launch_mxfp4_dequant(const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int64_t M, int64_t K,
                          void* out, int dtype, int64_t ld_out, hipStream_t stream) {
-  const Runs r = runs_of(M, K);
+  const int cus = cu_count();
+  if (cus <= 0) {
+    set_error("cannot query the CU count of the current device");
+    return CDIT_EHIP;
+  }
+  const Runs r = runs_of(M, K, cus);
   const dim3 grid = r.grid(M);
   const bool once = 2 * M * K > kOnceBytes;
 #define CDIT_MXD(DT, ONCE)                                                                                               \
