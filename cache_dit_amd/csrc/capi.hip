@@ -154,6 +154,9 @@ int cdit_debug_set_gemm_variant(int variant) {
   return prev;
 }
 
+static int64_t mx_scale_bytes(int64_t K) { return (K + 127) / 128 * 4; }
+constexpr int64_t kMxMostK = (int64_t)1 << 29;  // (the quantizer's grid; offsets inside a row in 32 bits)
+
 // A problem with contiguous, aligned operands; false: not one that an entry point takes.
 static bool shape_only(GemmArgs* g, int64_t M, int64_t N, int64_t K, int out_dtype_id) {
   if (M < 1 || N < 1 || K < 1 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX || out_dtype_id < CDIT_DT_F16 ||
@@ -178,6 +181,19 @@ int cdit_debug_gemm_choice(int weight_only, int64_t M, int64_t N, int64_t K, int
 int cdit_debug_linear_launches(int64_t M, int64_t N, int64_t K) {
   GemmArgs g;
   return shape_only(&g, M, N, K, CDIT_DT_BF16) ? linear_fp8_launches(g) : -1;
+}
+
+int cdit_debug_mxfp4_choice(int weight_only, int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 32 || K % 32 != 0 || K > kMxMostK || M > INT32_MAX - 512 || N > INT32_MAX - 512) return -1;
+  Mx4Gemm g = {};
+  g.M = (int)M;
+  g.N = (int)N;
+  g.K = (int)K;
+  g.lda = weight_only ? K : K / 2;
+  g.ldb = K / 2;
+  g.ldas = g.ldbs = mx_scale_bytes(K);
+  g.ldo = N;
+  return weight_only ? choose_gemm_w4a16(g) : choose_gemm_mxfp4(g);
 }
 
 int cdit_debug_set_quant_hints(int hints) {
@@ -636,10 +652,7 @@ int cdit_fp8_linear_w8a8(const void* x_bf16, const void* w_q, const float* w_sca
 
 // ---- MXFP4
 static bool known_dtype(int id) { return id == CDIT_DT_F16 || id == CDIT_DT_BF16 || id == CDIT_DT_F32; }
-static int64_t mx_scale_bytes(int64_t K) { return (K + 127) / 128 * 4; }
 static bool on(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
-
-constexpr int64_t kMxMostK = (int64_t)1 << 29;  // (the quantizer's grid; offsets inside a row in 32 bits)
 
 // A matrix in MXFP4: codes on `align` bytes.
 static int check_mx(const char* fn, const char* what, const void* codes, const void* scales, int64_t rows, int64_t K,

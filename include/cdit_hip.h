@@ -492,9 +492,13 @@ int cdit_debug_set_quant_hints(int hints);
  * cdit_debug_gemm_choice: the variant that cdit_fp8_gemm_rowwise runs (weight_only != 0:
  * cdit_w8a16_gemm, whose only output type is bf16).
  * cdit_debug_linear_launches: kernels that cdit_fp8_linear_w8a8 launches, 1 or 2.
+ * cdit_debug_mxfp4_choice: the variant that cdit_mxfp4_gemm runs for 16-bit outputs (weight_only != 0: cdit_w4a16_gemm): 0 the
+ * kernel without tiles, 1 256 x 256, 2 128 x 128, 3 64 x 128, 4 64 x 64, 5 128 x 256, 6 256 x 128, 7 128 x 64, 8 32 x 64 (rows x
+ * columns of a tile), 100 the kernel for few rows.
  */
 int cdit_debug_gemm_choice(int weight_only, int64_t M, int64_t N, int64_t K, int out_dtype_id);
 int cdit_debug_linear_launches(int64_t M, int64_t N, int64_t K);
+int cdit_debug_mxfp4_choice(int weight_only, int64_t M, int64_t N, int64_t K);
 
 /*
  * Measurement aid, not part of the operator interface (no counterpart in the reference):
