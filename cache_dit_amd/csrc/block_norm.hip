@@ -208,7 +208,8 @@ __device__ __forceinline__ void statistics(const Args& a, bool layer, Sum& sum, 
   *rstd = 1.0f / __fsqrt_rn(sum(s) * inv_k + a.eps);
 }
 
-// A workgroup per row, the row read again in each pass, value by value: rows of less than 8 values, or of more than 16384.
+// A workgroup per row, the row read again in each pass, value by value: rows of less than 8 values, or of more than 16384. us, 4096 x
+// 20000: bf16 1009 (0.65 TB/s), with an fp32 stream 1233 (0.8).
 template <int ST, int DT>
 __global__ __launch_bounds__(256) void gate_residual_norm_any(Args a) {
   __shared__ float slots[2][4];
@@ -239,9 +240,14 @@ __global__ __launch_bounds__(256) void gate_residual_norm_any(Args a) {
 
 // The row in registers: CH pieces per lane, WAVES wavefronts per row, 16-byte accesses. A workgroup takes a run of consecutive
 // rows; the next row's loads are under way while a row is worked on, and the vectors, folded into one factor of the branch and a
-// factor and an addend of the result, stay in registers until a row takes others (with one piece a lane; with two, where the
-// registers of 16 wavefronts would not hold them, each row reads them again from the caches). us, 32760 x 5120, fp32 stream,
-// one set of vectors: 604 with the vectors read for each row, 417 so (4.8 TB/s; a copy of 1 GiB runs at 5.1).
+// factor and an addend of the result, stay in registers until a row takes others (with one piece a lane; with two each row reads
+// them again from the caches). us, 32760 x 5120, fp32 stream, one set of vectors: 604 with the vectors read for each row, 406 so
+// (4.95 TB/s; a copy of 1 GiB runs at 5.1).
+//
+// Rows above 8192, two pieces a lane, spill nonetheless: the 128 registers of 16 wavefronts do not hold a row's h beside the next
+// row's loads (16 to 18 registers to scratch with 16-bit streams, 46 to 60 with fp32 ones), nor do the 168 of 12 with an fp32 stream
+// (6 to 14). us, bf16, and with an fp32 stream: 4096 x 8192 54 (4.96 TB/s) and 81 (4.98), x 12288 90 (4.5) and 145 (4.2), x 15360 112
+// (4.5) and 200 (3.8); unaligned, bf16, x 8192 52, x 15360 138.
 //
 // ANY: rows of any length from 8 on, wherever they start. The last piece ends with the row and begins with values of the piece
 // before it: these count once, and are stored twice, alike. us, bf16: 8192 x 5121 83 (5120: 70), 420 with the kernel above; 20000 x 71

@@ -39,7 +39,7 @@ __device__ __forceinline__ void locate(const Runs& r, uint32_t piece, uint32_t* 
 // ONCE: non-temporal accesses to the side that is not in 4 bits. For 16-bit types above 64 MB, us: quantizer 32760 x 5120 84.0 ->
 // 71.9 (5.9 TB/s), 32760 x 13824 213 -> 187 (6.15); inverse 83.7 -> 66.1 (6.4), 210 -> 165 (6.9). Below it makes no difference (4608
 // x 5120 11.4 and 11.3; 11.1 and 10.1); with fp32, where a lane's 32 bytes take two instructions on the same lines, it costs 20 to
-// 40 %.
+// 40 %. fp32 without: 4608 x 5120 16.9 (6.3) and 18.7 (5.7), 32760 x 5120 147 (5.2) and 200 (3.8).
 constexpr int64_t kOnceBytes = (int64_t)64 << 20;
 template <int DT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void mxfp4_quant_rows(const uint8_t* __restrict__ x, int64_t ld_x,
