@@ -86,12 +86,13 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_direct(Mx4Gemm g) {
 // (those of its own half; a row's 32 are one request), and byte permutations and a swap between the halves of the
 // wavefront bring them in order.
 //
-// Measured (M x N x K, weights and codes in HBM or caches as they come): 32760 x 13824 x 5120 in 256 x 256 tiles 1055 to 1080 us, 4.3
-// to 4.4 PFLOP/s, with GELU 1135, in fp32 (128 x 256 tiles) 1297; a loop of nothing but the instruction on random operands runs at 6.4 (the clock falls to 1.56 GHz), 725 us. Matrix cores
-// busy 65 % of the cycles, no LDS conflicts. With a part left out: no scales after a tile's first 1050, no LDS-DMA after three
-// steps 1110, no LDS reads 1045, no stores 1040, none of scales, DMA and reads 945: a wavefront a SIMD has nothing to cover a
-// tile's end (2.8 us) and a step's changes with. Two a SIMD (128 x 256) need 1.7 times the reads per product: 1225 us. Few tiles
-// are bound by what a CU takes from the caches, 50 to 60 GB/s: 512 x 5120 x 4096 in 128 x 128 tiles (160 of 256 CUs) 13.9 us.
+// Measured (M x N x K, weights and codes in HBM or caches as they come): 32760 x 13824 x 5120 in 256 x 256 tiles 1055 to 1080 us,
+// 4.3 to 4.4 PFLOP/s, with GELU 1135, in fp32 (128 x 256 tiles) 1297; a loop of nothing but the instruction on random operands runs
+// at 6.4 (the clock falls to 1.56 GHz), 725 us. Matrix cores busy 65 % of the cycles, no LDS conflicts. With a part left out: no
+// scales after a tile's first 1050, no LDS-DMA after three steps 1110, no LDS reads 1045, no stores 1040, none of scales, DMA and
+// reads 945 (of 1090): a wavefront a SIMD has nothing to cover a tile's end (2.8 us) and a step's changes with. Two a SIMD in tiles
+// of 128 x 256 need 1.7 times the reads per product: 1225 us. Few tiles are bound by what a CU takes in, 50 to 60 GB/s: 512 x 5120 x
+// 4096 in 128 x 128 tiles (160 of 256 CUs) 14 us.
 template <int BM_, int BN_, int WGM_, int WGN_, int SA_, int SB_, int WPE_>
 struct MxTile {
   static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, SA = SA_, SB = SB_, WPE = WPE_;

@@ -78,8 +78,8 @@ __global__ __launch_bounds__(256) void gemm_w4a16_direct(Mx4Gemm g) {
 //   line k + 1 (the codes of a line are read one step ahead)
 //
 // Measured: 4608 x 5120 x 5120 (M x N x K) 185 to 190 us, 1.27 to 1.30 PFLOP/s (256 x 128 tiles; 200 in 256 x 256, 191 in 128 x
-// 256), 16384 x 5120 x 5120 592 us, 1.45 (256 x 256 tiles); the
-// library's bf16 product reaches 1.36 on 16384 x 16384 x 16384. Bound by the matrix cores at the clock they run at.
+// 256), 16384 x 5120 x 5120 592 us, 1.45 (256 x 256 tiles); the library's bf16 product reaches 1.36 on 16384 x 16384 x 16384. Bound
+// by the matrix cores at the clock they run at.
 template <int BM_, int BN_, int WGM_, int WGN_, int SA_, int WPE_>
 struct W4Tile {
   static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, SA = SA_, SB = 2, WPE = WPE_;
