@@ -506,7 +506,9 @@ __global__ __launch_bounds__(256, KS <= 4 ? 2 : 1) void lora_up_rows(Args a, con
   const int64_t begin = (int64_t)blockIdx.y * columns, end = min(a.N, begin + columns);
 
   // base and out: rows 16 wave + 4 j + g, columns n0 + 8 i16. Aligned (out_aligned) as buffers, whose rows end with the
-  // tile's: what lies behind is zeros, and not stored.
+  // tile's: what lies behind is zeros, and not stored. All of an offset is in its vector register, here and wherever this file reads
+  // or writes through a buffer: that is what is compared with the buffer's size. A scalar offset is taken off the size first, and
+  // the rows of a short tile, or the columns behind N, can lie further than the size is: a difference below zero would bound nothing.
   auto buffer = [&](const void* p, int64_t ld) -> __amdgpu_buffer_rsrc_t {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(static_cast<const uint16_t*>(p) + row0 * ld), 0,
                                              (int)(((rows - 1) * ld + a.N) * 2), 0x00020000);
@@ -530,7 +532,7 @@ __global__ __launch_bounds__(256, KS <= 4 ? 2 : 1) void lora_up_rows(Args a, con
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const v4u v = __builtin_bit_cast(
-            v4u, __builtin_amdgcn_raw_buffer_load_b128(from, (int)base_at, (int)(n0 * 2 + 8 * j * a.ld_base), 0));
+            v4u, __builtin_amdgcn_raw_buffer_load_b128(from, (int)(base_at + (uint32_t)(n0 * 2 + 8 * j * a.ld_base)), 0, 0));
 #pragma unroll
         for (int i = 0; i < 4; ++i) b[j].w[i] = v[i];
       }
@@ -562,9 +564,9 @@ __global__ __launch_bounds__(256, KS <= 4 ? 2 : 1) void lora_up_rows(Args a, con
         if (r < rows && have > 0) store_out<true>(to + ((uint32_t)r * (uint32_t)a.ld_out + (uint32_t)n), have, y);
       } else {
         const v4u v = {y.w[0], y.w[1], y.w[2], y.w[3]};
-        // (The whole offset in a vector register. With a scalar one beside it the compiler holds the store to have read its data when
-        // it is issued and lets the next instruction write the first of these registers, which has reached memory: lanes 12 to 15 of
-        // each 16, where several workgroups share a CU.)
+        // (With a scalar offset the compiler also holds the store to have read its data when it is issued and lets the next
+        // instruction write the first of these registers, which has reached memory: lanes 12 to 15 of each 16, where several
+        // workgroups share a CU.)
         const uint32_t at = out_at + (uint32_t)(n0 * 2 + 8 * j * a.ld_out);
         __builtin_amdgcn_raw_buffer_store_b128(v, buffer(a.out, a.ld_out), (int)(have > 0 ? at : 0x80000000u), 0, 0);
       }
@@ -660,7 +662,7 @@ __global__ __launch_bounds__(256, KS <= 4 ? 2 : 1) void lora_up_rows(Args a, con
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       w[h] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(
-                                         up_buf, (int)up_at, (int)(((n0 + 4 * h) * a.R + (32 * k < rank ? 32 * k : 0)) * 2), 0));
+                                         up_buf, (int)(up_at + (uint32_t)(((n0 + 4 * h) * a.R + (32 * k < rank ? 32 * k : 0)) * 2)), 0, 0));
   };
   // (with the addresses that ANY needs, four pieces leave no registers for two columns of base at a time)
   constexpr bool LATE = ANY && KS == 4;
@@ -782,16 +784,16 @@ __global__ __launch_bounds__(256) void lora_down_tall(Args a, float* t, int k_pe
 #pragma unroll
       for (int n = 0; n < C::NX; ++n)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(x_buf, (__attribute__((address_space(3))) void*)(ring + stage + (wave + 4 * n) * 1024), 16,
-                                                 (int)(x_at[n] | behind), s * 128, 0, 0);
+                                                 (int)((x_at[n] + (uint32_t)s * 128) | behind), 0, 0, 0);
 #pragma unroll
       for (int half = 0; half < C::HALVES; ++half) {
-        const int k = (s * C::HALVES + half) * 128;  // bytes
-        const uint32_t behind = (uint32_t)k + 16 * chunk < w_ld ? 0u : 0x80000000u;
+        const uint32_t k = (uint32_t)(s * C::HALVES + half) * 128;  // bytes; of FP8's second half behind the row's end, maybe
+        const uint32_t behind = k + 16 * chunk < w_ld ? 0u : 0x80000000u;
 #pragma unroll
         for (int n = 0; n < C::NW; ++n)
           __builtin_amdgcn_raw_ptr_buffer_load_lds(
               w_buf, (__attribute__((address_space(3))) void*)(ring + stage + C::X_BYTES + half * C::W_BYTES + w_block(n) * 1024), 16,
-              (int)(w_at[n] | behind), k, 0, 0);
+              (int)((w_at[n] + k) | behind), 0, 0, 0);
       }
     };
     v4f acc[MT][RW];
