@@ -82,11 +82,17 @@ def _lora_add(base, x, down, up, ids, scale, rank, x_scale, epilogue=0):
   up = up.contiguous()
   up = up if up.data_ptr() % 16 == 0 else up.clone()
   lead = base.shape[:-1]
-  ids = ids.reshape(-1, 1).expand(-1, rows // ids.numel()).reshape(rows) if x.dim() != 2 else ids
-  base2 = base if base.dim() == 2 and base.stride(1) == 1 and N <= base.stride(0) < 1 << 24 else base.contiguous().view(rows, N)
-  x2 = x if x.dim() == 2 and x.stride(1) == 1 and K <= x.stride(0) < 1 << 24 else x.contiguous().view(rows, K)
-  out = _results(launch(base2, x2, down.contiguous(), up, ids, scale, rank, x_scale, epilogue))[0]
-  return out.view(*lead, N)
+  if x.dim() == 2:
+    base = base if base.stride(1) == 1 and N <= base.stride(0) < 1 << 24 else base.contiguous().view(rows, N)
+    x = x if x.stride(1) == 1 and K <= x.stride(0) < 1 << 24 else x.contiguous().view(rows, K)
+  else:  # as many rows for each of the ids
+    ids = ids.reshape(-1)
+    base = base.contiguous().view(ids.numel(), -1, N)
+    x = x.contiguous().view(ids.numel(), -1, K)
+  launched = launch(base, x, down.contiguous(), up, ids, scale, rank, x_scale, epilogue)
+  if launched is None:
+    raise RuntimeError(f"{name}: arguments that were laid out for the kernels were not taken")
+  return _results(launched)[0].view(*lead, N)
 
 
 torch.library.impl("cdit::lora_add", "CUDA")(_lora_add)

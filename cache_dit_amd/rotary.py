@@ -99,7 +99,10 @@ def _rotary_general(q, k, positions, inv_freq, cos, sin, q_weight, k_weight, lay
             *_rotary_general(k, None, positions, inv_freq, cos, sin, weights[1], None, layout, ends, scale, eps)]
   q = q if q.stride(-1) == 1 else q.contiguous()
   k = k if k is None or k.stride(-1) == 1 else k.contiguous()
-  return list(_results(launch(q, k, positions, inv_freq, cos, sin, *weights, layout, ends, scale, eps)))
+  launched = launch(q, k, positions, inv_freq, cos, sin, *weights, layout, ends, scale, eps)
+  if launched is None:
+    raise RuntimeError(f"{name}: arguments that were laid out for the kernels were not taken")
+  return list(_results(launched))
 
 
 torch.library.impl("cdit::rotary_embed", "CUDA")(_rotary_general)
