@@ -576,8 +576,9 @@ __global__ __launch_bounds__(256, KS <= 4 ? 2 : 1) void lora_up_rows(Args a, con
   Mx8<CDIT_DT_BF16> next[4];
   fetch(begin, next);
   if (count != 1) {
-    // Any number of adapters: one piece of 32 ranks after the other, whichever adapter's it is, and each row takes its own's. kAhead
-    // pieces are under way, the next columns' among them.
+    // Any number of adapters: one piece of 32 ranks after the other, whichever adapter's it is, and each row takes its own's. The sum
+    // goes through the instructions as in a tile of one adapter: a row's result has the same bits whatever the rows beside it name.
+    // kAhead pieces are under way, the next columns' among them.
     constexpr int kAhead = 4;
     const int pieces_of_up = __builtin_amdgcn_readfirstlane(tile.parts);
     v4f acc[4][2];
@@ -626,11 +627,10 @@ __global__ __launch_bounds__(256, KS <= 4 ? 2 : 1) void lora_up_rows(Args a, con
           const bool member = members >> (16 * m + i16) & 1;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            v4f d = {0, 0, 0, 0};
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w[i][h]), hi, d, 0, 0, 0);
+            v4f d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w[i][h]), hi, acc[m][h], 0, 0, 0);
             d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w[i][h]), lo, d, 0, 0, 0);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) acc[m][h][q] = member ? acc[m][h][q] + d[q] : acc[m][h][q];
+            for (int q = 0; q < 4; ++q) acc[m][h][q] = member ? d[q] : acc[m][h][q];
           }
         }
         load(w[i]);
