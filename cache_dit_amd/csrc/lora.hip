@@ -259,6 +259,12 @@ __device__ __forceinline__ void split4(const v4f& x, uint16_t* upper, uint16_t* 
   *reinterpret_cast<v2u*>(upper) = v2u{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
   *reinterpret_cast<v2u*>(lower) = v2u{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3])};
 }
+// The 8 places behind a row's R ranks, which are what an operand of 32 ranks finds where R ends in its middle. Zeros: up's operand is
+// cut to zeros there as well, but zero times an infinity of another rank would be a NaN.
+__device__ __forceinline__ void clear_behind(const Args& a, int rows, uint16_t* upper, uint16_t* lower) {
+  const int m = (int)threadIdx.x % rows;
+  if ((int)threadIdx.x < 2 * rows) *reinterpret_cast<v4u*>(((int)threadIdx.x < rows ? upper : lower) + m * (a.R + 8) + a.R) = v4u{0, 0, 0, 0};
+}
 __device__ __forceinline__ int stage_t(const Args& a, const float* t, int pieces, int64_t row0, int rows, Tile& tile, uint16_t* upper,
                                        uint16_t* lower) {
   const int lane = threadIdx.x & 63, ld = a.R + 8;
@@ -290,6 +296,7 @@ __device__ __forceinline__ int stage_t(const Args& a, const float* t, int pieces
     if ((int)threadIdx.x == count - 1) tile.parts = at + here;
   }
   if (threadIdx.x == 0 && count == 0) tile.parts = 0;
+  clear_behind(a, 64, upper, lower);
   // quads of a row are a multiple of 4: 16 threads of a wavefront and more are in one row, or rows next to one another
   const int quads = a.R / 4, all = 64 * quads;
   constexpr int kBatch = 4;
@@ -419,6 +426,7 @@ __global__ __launch_bounds__(256) void lora_up(Args a, const float* t, int piece
       for (int i = 0; i < kAhead; ++i) load(w[i]);
     }
     if (steps > 0) {
+      clear_behind(a, 16, upper, lower);
       const int quads = a.R / 4;
       for (int q = threadIdx.x; q < 16 * quads; q += 256) {
         const int m = (int)((uint32_t)q / (uint32_t)quads), r = 4 * (q - m * quads);
@@ -462,7 +470,7 @@ __global__ __launch_bounds__(256) void lora_up(Args a, const float* t, int piece
       for (int i = 0; i < kAhead; ++i) {
         if (n0 >= end) break;
         cut_up(rank, 32 * k, w[i]);
-        const int at = i16 * ld + min(32 * k + 8 * g, a.R - 8);  // (behind R: up's operand is 0)
+        const int at = i16 * ld + min(32 * k + 8 * g, a.R);  // (behind R: zeros)
         const v8bf hi = *reinterpret_cast<const v8bf*>(upper + at), lo = *reinterpret_cast<const v8bf*>(lower + at);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -622,7 +630,7 @@ __global__ __launch_bounds__(256, KS <= 4 ? 2 : 1) void lora_up_rows(Args a, con
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           if (!(__builtin_amdgcn_readfirstlane((int)(members >> (16 * m))) & 0xffff)) continue;
-          const int at = (16 * m + i16) * (a.R + 8) + min(k + 8 * g, a.R - 8);  // (behind R: up's operand is 0)
+          const int at = (16 * m + i16) * (a.R + 8) + min(k + 8 * g, a.R);  // (behind R: zeros)
           const v8bf hi = *reinterpret_cast<const v8bf*>(upper + at), lo = *reinterpret_cast<const v8bf*>(lower + at);
           const bool member = members >> (16 * m + i16) & 1;
 #pragma unroll
@@ -649,7 +657,7 @@ __global__ __launch_bounds__(256, KS <= 4 ? 2 : 1) void lora_up_rows(Args a, con
   for (int m = 0; m < 4; ++m)
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      const int at = (16 * m + i16) * (a.R + 8) + min(32 * k + 8 * g, a.R - 8);  // (behind R: up's operand is 0)
+      const int at = (16 * m + i16) * (a.R + 8) + min(32 * k + 8 * g, a.R);  // (behind R: zeros)
       hi[m][k] = *reinterpret_cast<const v8bf*>(upper + at);
       lo[m][k] = *reinterpret_cast<const v8bf*>(lower + at);
     }
