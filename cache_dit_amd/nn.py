@@ -92,9 +92,15 @@ class _Fp8LinearBase(nn.Linear):
     return self.epilogue if self._adapters() is None else _native.EPI_NONE
 
   def _with_adapters(self, out: torch.Tensor, x) -> torch.Tensor:
-    """`out`, the projection of x, with what the adapters of x's rows add."""
+    """`out`, the projection of x, with what the adapters of x's rows add. Of an activation without bf16 values
+    (ln_modulate_quant(materialize=False)) they take the codes that the projection took."""
     lora = self._adapters()
-    return out if lora is None else lora(out, x, self.epilogue)
+    if lora is None:
+      return out
+    if not isinstance(x, tuple) and not torch.compiler.is_compiling() and ops.is_codes_only(x):
+      q, s = ops.shared_activation_quant(ops._as_rows(x), self._scale_mode_id)
+      x = q.view(x.shape), s.view(*x.shape[:-1], 1)
+    return lora(out, x, self.epilogue)
 
   def extra_repr(self) -> str:
     return (f"in_features={self.in_features}, out_features={self.out_features}, "
