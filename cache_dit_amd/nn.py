@@ -653,6 +653,8 @@ def linear_on_cat(linear: nn.Module, xs) -> torch.Tensor:
       and all(x.is_cuda and x.dtype == torch.bfloat16 for x in xs)):
     return ops.linear_w8a8_cat2_op(xs[0], xs[1], linear.weight, linear.weight_scale,
                                    linear.bias, linear._scale_mode_id, linear.epilogue)
+  if not torch.compiler.is_compiling():
+    ops._reject_codes_only("linear_on_cat", *xs)
   return linear(torch.cat(xs, dim=-1))
 
 
