@@ -203,7 +203,8 @@ def rotary_frequencies(rot: int, theta: float = 10000.0, *, scaling: Optional[st
   elif scaling == "yarn":
     def index_of(turns):  # theta^(-2i / rot) original_length = 2 pi turns
       return rot * math.log(original_length / (2 * math.pi * turns)) / (2 * math.log(theta))
-    first, last = max(math.floor(index_of(high)), 0), min(math.ceil(index_of(low)), rot // 2 - 1)
+    # (the ramp may end behind the last pair: its upper end is kept within the dimensions, not the pairs)
+    first, last = max(math.floor(index_of(high)), 0), min(math.ceil(index_of(low)), rot - 1)
     kept = 1 - ((index - first) / max(last - first, 0.001)).clamp(0, 1)
     freq = freq * (kept + (1 - kept) / factor)
     scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
