@@ -87,6 +87,9 @@ class _Fp8LinearBase(nn.Linear):
     lora = self._modules.get("lora")
     return None if lora is None or lora.ids is None else lora
 
+  # A Linear without children has no adapters, and its call does not pay for them: two calls of the methods below are a microsecond
+  # of the eight or so that a small Linear takes on the host.
+
   def _own_epilogue(self) -> int:
     """What the projection itself applies: behind adapters, the activation comes with them."""
     return self.epilogue if self._adapters() is None else _native.EPI_NONE
@@ -181,7 +184,8 @@ class SiblingGroup:
         self.drop_pending()
         if _pending_group is self:
           _pending_group = None
-      return lin._with_adapters(out.view(*x.shape[:-1], lin.out_features), x)
+      out = out.view(*x.shape[:-1], lin.out_features)
+      return lin._with_adapters(out, x) if lin._modules else out
     # A group that computes afresh while another still holds uncollected outputs: that
     # forward left its siblings early (an exception, a skipped branch); its leftovers (up to
     # M x sum(N) bf16) are released here rather than kept until its next call.
@@ -193,15 +197,16 @@ class SiblingGroup:
     outs = [torch.empty((M, m.out_features), dtype=torch.bfloat16, device=x2.device) for m in members]
     if M > 0 and self.weight_only:
       ops.w8a16_batched_into([(x2, [m.weight for m in members], [m.weight_scale for m in members],
-                               [m.bias for m in members], outs, [m._own_epilogue() for m in members])])
+                               [m.bias for m in members], outs, [m._own_epilogue() if m._modules else m.epilogue for m in members])])
     elif M > 0:
       q, s = ops.shared_activation_quant(x2, lin._scale_mode_id)
       ops.gemm_rowwise_grouped_into(q, s, [m.weight for m in members],
                                     [m.weight_scale for m in members], [m.bias for m in members],
-                                    outs, [m._own_epilogue() for m in members])
+                                    outs, [m._own_epilogue() if m._modules else m.epilogue for m in members])
     out, outs[i] = outs[i], None
     self.key, self.outs, self.capture_id, self.stream = _InputKey(x2), outs, capture_id, stream
-    return lin._with_adapters(out.view(*x.shape[:-1], lin.out_features), x)
+    out = out.view(*x.shape[:-1], lin.out_features)
+    return lin._with_adapters(out, x) if lin._modules else out
 
 
 #: the sibling group whose outputs are waiting to be collected, if any (one at a time: the
@@ -256,8 +261,8 @@ class Fp8DynamicLinear(_Fp8LinearBase):
     if isinstance(x, tuple):
       codes, scales = x
       out = ops.float8_inference_scaled_mm(codes, scales, self.weight.t(), self.weight_scale, torch.bfloat16,
-                                           bias=self.bias, epilogue=self._own_epilogue())
-      return self._with_adapters(out, x)
+                                           bias=self.bias, epilogue=self._own_epilogue() if self._modules else self.epilogue)
+      return self._with_adapters(out, x) if self._modules else out
     self._check_input(x)
     # sharing and grouping keep state between calls (the last activation's codes, the
     # siblings' outputs); a compiled graph gets the stateless form (its front end owns the
@@ -268,7 +273,7 @@ class Fp8DynamicLinear(_Fp8LinearBase):
       if self._precomputed is not None:
         out = _take_precomputed_traced(self, x)
         if out is not None:
-          return self._with_adapters(out, x)
+          return self._with_adapters(out, x) if self._modules else out
     else:
       if x.is_inference():
         if self.sibling_group is not None or self.share_input_quant:
@@ -277,15 +282,15 @@ class Fp8DynamicLinear(_Fp8LinearBase):
         if self._precomputed is not None:
           out = _take_precomputed(self, x)
           if out is not None:
-            return self._with_adapters(out, x)
+            return self._with_adapters(out, x) if self._modules else out
         if _recorder is not None:
           _recorder.note(self, x)
         if self.sibling_group is not None:
           return self.sibling_group.forward_member(self, x)
     share = self.share_input_quant and not stateless
     out = ops.linear_w8a8_op(x, self.weight, self.weight_scale, self.bias, self._scale_mode_id,
-                             self._own_epilogue(), ops.GRANULARITY_PER_ROW, share)
-    return self._with_adapters(out, x)
+                             self._own_epilogue() if self._modules else self.epilogue, ops.GRANULARITY_PER_ROW, share)
+    return self._with_adapters(out, x) if self._modules else out
 
 
 class Fp8DynamicLinearPerTensor(_Fp8LinearBase):
@@ -297,8 +302,8 @@ class Fp8DynamicLinearPerTensor(_Fp8LinearBase):
   def forward(self, x: torch.Tensor) -> torch.Tensor:
     self._check_input(x)
     out = ops.linear_w8a8_op(x, self.weight, self.weight_scale, self.bias, self._scale_mode_id,
-                             self._own_epilogue(), ops.GRANULARITY_PER_TENSOR, False)
-    return self._with_adapters(out, x)
+                             self._own_epilogue() if self._modules else self.epilogue, ops.GRANULARITY_PER_TENSOR, False)
+    return self._with_adapters(out, x) if self._modules else out
 
 
 class Fp8WeightOnlyLinear(_Fp8LinearBase):
@@ -313,7 +318,7 @@ class Fp8WeightOnlyLinear(_Fp8LinearBase):
       if self._precomputed is not None:
         out = _take_precomputed_traced(self, x)
         if out is not None:
-          return self._with_adapters(out, x)
+          return self._with_adapters(out, x) if self._modules else out
     else:
       if x.is_inference():
         if self.sibling_group is not None:
@@ -322,14 +327,14 @@ class Fp8WeightOnlyLinear(_Fp8LinearBase):
         if self._precomputed is not None:
           out = _take_precomputed(self, x)
           if out is not None:
-            return self._with_adapters(out, x)
+            return self._with_adapters(out, x) if self._modules else out
         if _recorder is not None:
           _recorder.note(self, x)
         if self.sibling_group is not None:
           return self.sibling_group.forward_member(self, x)
     out = ops.w8a16_mm_op(x, self.weight.t(), self.weight_scale, self.bias, _native.DT_BF16,
-                          self._own_epilogue())
-    return self._with_adapters(out, x)
+                          self._own_epilogue() if self._modules else self.epilogue)
+    return self._with_adapters(out, x) if self._modules else out
 
 
 class Mxfp4Linear(_Fp8LinearBase):
@@ -344,11 +349,12 @@ class Mxfp4Linear(_Fp8LinearBase):
   def forward(self, x):
     if isinstance(x, tuple):
       codes, scales = x
-      out = mxfp4.mxfp4_mm(codes, scales, self.weight, self.weight_scale, torch.bfloat16, self.bias, self._own_epilogue())
-      return self._with_adapters(out, x)
+      out = mxfp4.mxfp4_mm(codes, scales, self.weight, self.weight_scale, torch.bfloat16, self.bias,
+                           self._own_epilogue() if self._modules else self.epilogue)
+      return self._with_adapters(out, x) if self._modules else out
     self._check_input(x)
-    out = mxfp4.mxfp4_linear_op(x, self.weight, self.weight_scale, self.bias, self._own_epilogue())
-    return self._with_adapters(out, x)
+    out = mxfp4.mxfp4_linear_op(x, self.weight, self.weight_scale, self.bias, self._own_epilogue() if self._modules else self.epilogue)
+    return self._with_adapters(out, x) if self._modules else out
 
 
 class Mxfp4WeightOnlyLinear(_Fp8LinearBase):
@@ -357,8 +363,8 @@ class Mxfp4WeightOnlyLinear(_Fp8LinearBase):
 
   def forward(self, x: torch.Tensor) -> torch.Tensor:
     self._check_input(x)
-    out = mxfp4.w4a16_mm_op(x, self.weight, self.weight_scale, self.bias, self._own_epilogue())
-    return self._with_adapters(out, x)
+    out = mxfp4.w4a16_mm_op(x, self.weight, self.weight_scale, self.bias, self._own_epilogue() if self._modules else self.epilogue)
+    return self._with_adapters(out, x) if self._modules else out
 
 
 _CLASS_OF = {
@@ -505,7 +511,7 @@ def linear_batch(pairs):
   if plain:
     return [[lin(x) for lin in lins] for x, lins in pairs]
   outs = _batch(pairs)
-  if all(lin._adapters() is None for lin in flat):
+  if not any(lin._modules for lin in flat):
     return outs
   return [[lin._with_adapters(y, x) for lin, y in zip(lins, ys)] for (x, lins), ys in zip(pairs, outs)]
 
@@ -520,7 +526,7 @@ def _batch(pairs):
           else torch.ops.cdit.linear_w8a8_batch)
     args = ([x for x, _ in pairs], [lin.weight for lin in flat],
             [lin.weight_scale.reshape(-1) for lin in flat], [lin.bias for lin in flat],
-            [len(lins) for _, lins in pairs], [lin._own_epilogue() for lin in flat])
+            [len(lins) for _, lins in pairs], [lin._own_epilogue() if lin._modules else lin.epilogue for lin in flat])
     outs = op(*args) if type(first) is Fp8WeightOnlyLinear else op(*args, first._scale_mode_id)
     result, p = [], 0
     for _, lins in pairs:
@@ -537,7 +543,7 @@ def _batch(pairs):
       continue
     rows.append(x2)
     acts.append([None, None, [lin.weight for lin in lins], [lin.weight_scale for lin in lins],
-                 [lin.bias for lin in lins], outs, [lin._own_epilogue() for lin in lins]])
+                 [lin.bias for lin in lins], outs, [lin._own_epilogue() if lin._modules else lin.epilogue for lin in lins]])
   if acts and type(first) is Fp8WeightOnlyLinear:
     ops.w8a16_batched_into([(x2, *act[2:]) for x2, act in zip(rows, acts)])
   elif acts:
@@ -649,7 +655,8 @@ def linear_on_cat(linear: nn.Module, xs) -> torch.Tensor:
   Bit-identical to the plain expression, which is what runs for any other module, number of
   sources or dtype."""
   xs = list(xs)
-  if (type(linear) is Fp8DynamicLinear and len(xs) == 2 and linear.sibling_group is None and linear._adapters() is None
+  if (type(linear) is Fp8DynamicLinear and len(xs) == 2 and linear.sibling_group is None
+      and (not linear._modules or linear._adapters() is None)
       and all(x.is_cuda and x.dtype == torch.bfloat16 for x in xs)):
     return ops.linear_w8a8_cat2_op(xs[0], xs[1], linear.weight, linear.weight_scale,
                                    linear.bias, linear._scale_mode_id, linear.epilogue)
