@@ -492,9 +492,10 @@ def linear_batch(pairs):
   (encoder, [add_q_proj, add_k_proj, add_v_proj])]). Returns the outputs in the same
   nesting, bit-identical to calling the Linears one by one. For block forwards that are
   written against this package; `float8_per_row` Linears (one quantizer launch for the
-  stage as well) or `float8_weight_only` ones; other Linears, mixed types or inference-mode
-  tensors simply run one by one. Inside a compiled graph the stage is one traceable op
-  (`cdit::linear_w8a8_batch` / `cdit::w8a16_batch`) without the shared-quantization state."""
+  stage as well) or `float8_weight_only` ones; other Linears, mixed types, inference-mode
+  tensors or activations that are (codes, scales) already simply run one by one. Inside a
+  compiled graph the stage is one traceable op (`cdit::linear_w8a8_batch` /
+  `cdit::w8a16_batch`) without the shared-quantization state."""
   flat = [lin for _, lins in pairs for lin in lins]
   first = flat[0]
   plain = (len(flat) > _native.MAX_GROUP
@@ -502,7 +503,7 @@ def linear_batch(pairs):
            or type(first) not in (Fp8DynamicLinear, Fp8WeightOnlyLinear)
            or any(type(lin) is not type(first) or lin.in_features != first.in_features
                   or lin._scale_mode_id != first._scale_mode_id for lin in flat)
-           or any(not x.is_cuda or x.dtype != torch.bfloat16 for x, _ in pairs))
+           or any(isinstance(x, tuple) or not x.is_cuda or x.dtype != torch.bfloat16 for x, _ in pairs))
   compiling = torch.compiler.is_compiling()
   if not plain and not compiling:  # (no version counters on inference tensors: nothing is shared)
     plain = any(x.is_inference() for x, _ in pairs)
@@ -594,7 +595,7 @@ def _stage_batchable(pairs, flat, first, traced: bool) -> bool:
              or lin._scale_mode_id != first._scale_mode_id or lin.sibling_group is not None
              for lin in flat)):
     return False
-  return not any(not x.is_cuda or x.dtype != torch.bfloat16 or x.shape[-1] != first.in_features
+  return not any(isinstance(x, tuple) or not x.is_cuda or x.dtype != torch.bfloat16 or x.shape[-1] != first.in_features
                  or (not traced and x.is_inference()) for x, _ in pairs)
 
 
@@ -608,8 +609,8 @@ def precompute_stage(pairs) -> bool:
   it is. A Linear that is called with anything else computes as usual, so a wrong guess
   costs time, not correctness. Outputs nobody collects are dropped when the next stage is
   precomputed. Returns False (nothing done) where linear_batch would not batch:
-  inference-mode tensors, Linears of other types or of mixed types. Inside a traced graph
-  (torch.compile) the stage becomes the one traceable batch op and an output goes to the
+  inference-mode tensors, (codes, scales), Linears of other types or of mixed types. Inside a
+  traced graph (torch.compile) the stage becomes the one traceable batch op and an output goes to the
   Linear call that receives the same tensor object; whoever stashes there also clears what
   is left (`release_precomputed`). Not thread-safe, like the sibling groups."""
   flat = [lin for _, lins in pairs for lin in lins]

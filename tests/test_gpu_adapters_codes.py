@@ -36,6 +36,7 @@ def test_adapters_take_the_codes_too(cd):  # noqa: F811
   same([lin(y.view(42, 256).view(2, 21, 256)) for lin in lins])
   y, _ = activation(cd)
   same(cd.linear_batch([(y, lins)])[0])
+  same(cd.linear_batch([(codes, lins)])[0])
   y, _ = activation(cd)
   assert cd.precompute_stage([(y, lins)])
   same([lin(y) for lin in lins])
