@@ -117,7 +117,8 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.
   the ranks that are used of them (what lies behind is never looked at), scale [adapters] the adapters' strengths. ids, whole
   numbers: one for each index of x's first dimensions ([batch] for x [batch, tokens, K], or one a row), or one for all.
   Rows of one adapter next to one another are the fast case, any order is right. Sums are held in fp32, x down^T is carried on with
-  16 bits, the result is rounded once. For inference: a tensor that requires a gradient is refused while gradients are recorded."""
+  16 bits, the result is rounded once; a row's result has the same bits whatever the rows beside it name. up holds finite numbers.
+  For inference: a tensor that requires a gradient is refused while gradients are recorded."""
   name = "lora_add"
   grad = torch.is_grad_enabled()
   tensors = (base, x, down, up, ids, scale, rank, x_scale)

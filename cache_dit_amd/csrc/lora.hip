@@ -9,9 +9,11 @@
 // order: a tile is multiplied by every adapter that its rows name, and each row keeps what its own gave. Rows of one request next to
 // one another make tiles of one adapter; a tile of single tokens reads each of their adapters, which it has to.
 //
-// us, first and second product: one row, 5120 x 13824, rank 16: 4.4 and 4.6 (a launch and a step's latency each); 64 rows, 5120 x 5120, 24
-// adapters up to rank 64: 8.7 and 10.4 (20 MB of adapters, 1 TB/s: a CU takes in some 100 GB/s); 16384 x 2560 x 10240, rank 32, GELU: 24
-// to 32 and 139 to 157 (671 MB, 4.3 to 4.8 TB/s); codes, 32760 x 5120 x 5120, ranks 128 and 64: 67 and 166 (4.0 TB/s).
+// us, first and second product, the median of a kernel trace's passes (their fastest): one row, 5120 x 13824, rank 16: 4.5 (4.2) and 5.5
+// (4.4), a launch and a step's latency each; 64 rows, 5120 x 5120, 24 adapters up to rank 64: 9.7 (8.0) and 11.2 (10.5), 9 MB of adapters
+// each at 1 TB/s, reads that wait for one another: ids, ranks, x and down; ids, ranks, the parts of t; 16384 x 2560 x 10240, rank 32,
+// GELU: 33 (24) and 158 (140), 671 MB at 4.2 TB/s (4.8); codes, 32760 x 5120 x 5120, ranks 128 and 64: 81 (67) and 190 (166), of which the
+// second moves 671 MB at 3.5 TB/s (4.0).
 //
 // Sums are held in fp32. t enters the second product as the sum of two bf16 numbers: the upper 16 bits of the fp32 number and,
 // rounded to bf16, what they leave out: 2^-16 of t. A single bf16 (2^-9) would cost as much as out's own rounding again.
@@ -126,8 +128,8 @@ __device__ __forceinline__ void for_groups(int mine, bool without, int slots, in
 }
 
 // t of few rows: of 64, the rows of one adapter, 16 at a time, and, for each group of four wavefronts, 16 RT ranks; the four take
-// every fourth step of the workgroup's piece of K and add up through LDS. A step's loads take a microsecond to come and one CU reads no
-// more than some 100 GB/s: an adapter's rows are read once for 64 rows, and K, ranks and adapters (slots) spread over all CUs.
+// every fourth step of the workgroup's piece of K and add up through LDS. A step's loads take a microsecond to come: an adapter's rows
+// are read once for 64 rows, and K, ranks and adapters (slots) spread over all CUs, so that few steps follow one another.
 // grid: 64 rows, pieces of K times slots, ranks.
 template <bool FP8, bool ANY, int RT>
 __global__ __launch_bounds__(512, RT == 4 ? 3 : 4) void lora_down(Args a, float* t, int steps_per_piece, int slots) {
@@ -924,10 +926,11 @@ __global__ __launch_bounds__(256) void lora_down_tall(Args a, float* t, int k_pe
 }
 
 // Up to 8 rows a CU count as few; in the first product with more than 32 ranks, or rows that cannot come by DMA, up to one. us, gathered
-// and in tiles, 5120 x 5120, 11 requests with 5 adapters: first product, 32 ranks, 300 rows 6.3 and 7.0, 1000 rows 9.4 and 12.0, 2000
-// rows 13.8 and 17.0; 64 ranks 8.4 and 8.4, 14.4 and 14.7, 22.6 and 20.6; 128 ranks 12.7 and 10.6, 28.5 and 19.3, 41.6 and 25.6; 16
-// ranks of 5121 x 5121 8.8 and 8.3, 17.9 and 11.5, 29 and 16. Second product, 32 ranks 10.8 and 16.0, 14.1 and 20.0, 22.3 and 23.4, 4096
-// rows 69 and 43; 128 ranks 17.9 and 32.6, 25.5 and 39.2, 35.7 and 45.5.
+// and in tiles, of 300, 1000, 2000 and 4096 rows, 11 requests with 5 adapters, 5120 x 5120. First product: 32 ranks 6.2 and 7.1, 9.6 and
+// 12.0, 13.7 and 12.6, 25 and 21; 64 ranks 8.9 and 8.4, 14.8 and 14.8, 21 and 16, 36 and 24; 128 ranks 14 and 10, 31 and 20, 43 and 21, 70
+// and 30; 16 ranks of 5121 x 5121 8.4 and 8.2, 19 and 11, 28 and 16, 41 and 32. Second product: 32 ranks 7.9 and 16, 14 and 20, 18 and 24,
+// 36 and 31; 64 ranks 11 and 20, 20 and 26, 28 and 32, 54 and 41; 128 ranks 16 and 34, 29 and 42, 40 and 50, 79 and 63; 16 ranks of 5121 x
+// 5121 8.6 and 15, 18 and 20, 28 and 25, 52 and 37.
 constexpr int64_t kFewRows = 8;
 struct Plan {
   int rt, groups, pieces, steps_per_piece;

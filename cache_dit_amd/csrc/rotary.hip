@@ -6,9 +6,10 @@
 //   (a, b) -> scale (a cos t - b sin t, a sin t + b cos t),  t = position[axis of the pair] * inv_freq[pair]
 //
 // The angles are not read from a table that grows with the context but made here, once per token and pair, and used for
-// all heads: the position times the frequency in turns, in fp64, so that what is left behind the whole turns is exact to
-// 2^-52 of the angle (at position 2^20 and frequency 1 to 4e-11 of a turn; in fp32 it would be 2 % of one). sine and cosine of
-// the rest, at most an eighth of a turn, are their Taylor series in fp32.
+// all heads: the position times the frequency in turns, in fp64 (three roundings), so that what is left behind the whole turns is
+// exact to 2^-51 of the angle (at position 2^20 and frequency 1 to 7e-11 of a turn; in fp32 it would be 2 % of one). The rest, at
+// most an eighth of a turn, is rounded to fp32, 2^-24 of it, and its sine and cosine are their Taylor series in fp32: what an output in
+// fp32 loses to that is a unit or two in its last place, and one in 16 bits nothing.
 #include <algorithm>
 
 #include "gemm_common.h"

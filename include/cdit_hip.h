@@ -481,7 +481,7 @@ int cdit_gate_residual_norm_fp8(const cdit_gate_residual_norm_args* args, void* 
  * Pairs: (v[i], v[i + rot / 2]) or (v[2i], v[2i + 1]). Pair i has t = position * inv_freq[i] (fp64, in radians), the position
  * of its axis: axis j has the pairs below section_end[j] that no axis before it has, the last one the rest. In place of
  * inv_freq and positions, cos and sin may be given, fp32 [B, S, rot / 2] with any strides. The products are made in fp64 and
- * reduced there: an angle is off by 2^-52 of it. All else in fp32; out is rounded once. Any stride and alignment is taken; D
+ * reduced there: an angle is off by 2^-51 of it at most. All else in fp32; out is rounded once. Any stride and alignment is taken; D
  * is at most 512; out must not overlap x.
  */
 enum cdit_rotary_layout { CDIT_ROTARY_HALF = 0, CDIT_ROTARY_INTERLEAVED = 1 };
@@ -518,7 +518,10 @@ int cdit_rotary(const cdit_rotary_args* args, void* stream);
  * down [adapters, R, K] and up [adapters, N, R] bf16, contiguous, R a multiple of 16 up to 256; of adapter i the first
  * rank[i] rows of down[i] and columns of up[i] are used (rank NULL: all R) and the others never looked at. scale
  * [adapters] fp32, NULL: 1. ids int32 or int64 (ids64). M below 2^29, K and N below 2^22, strides below 2^24.
- * Rows may name adapters in any order; rows next to one another that name one are the fast case. Sums in fp32; x down^T is carried on with 16 bits of significand (2^-16) and more; out is rounded once.
+ * Rows may name adapters in any order; rows next to one another that name one are the fast case. Sums in fp32, in an order that the
+ * shapes alone decide; x down^T is carried on with 16 bits of significand (2^-16) and more; GELU's exponential and reciprocal are the
+ * hardware's (2^-18 of the result); out is rounded once. up holds finite numbers: an infinity times one part of x down^T and the other
+ * can be a NaN.
  *
  * workspace: cdit_lora_workspace_bytes(M, K, R) bytes on the device at least, at 16 bytes (-1: no such problem, or no device).
  */
