@@ -32,7 +32,7 @@ torch.library.define(
 def _check_per_token(name, what, t, q, last):
   """[S] or [B, S] tokens of q [B, S, H, D] or [S, H, D], and `last` values for each (None: one)."""
   lead = t.shape if last is None else t.shape[:-1]
-  if (last is not None and t.shape[-1] != last) or lead not in (q.shape[:-2], q.shape[-3:-2]):
+  if (last is not None and t.shape[-1:] != (last, )) or lead not in (q.shape[:-2], q.shape[-3:-2]):
     tail = "" if last is None else f" with {last} values each"
     raise ValueError(f"{name}: {what} {tuple(t.shape)} for q {tuple(q.shape)}: expected one for each token "
                      f"{tuple(q.shape[:-2])} or {tuple(q.shape[-3:-2])}{tail}")
