@@ -518,7 +518,8 @@ __global__ __launch_bounds__(256, KS <= 4 ? 2 : 1) void lora_up_rows(Args a, con
   // base and out: rows 16 wave + 4 j + g, columns n0 + 8 i16. Aligned (out_aligned) as buffers, whose rows end with the
   // tile's: what lies behind is zeros, and not stored. All of an offset is in its vector register, here and wherever this file reads
   // or writes through a buffer: that is what is compared with the buffer's size. A scalar offset is taken off the size first, and
-  // the rows of a short tile, or the columns behind N, can lie further than the size is: a difference below zero would bound nothing.
+  // the rows of a short tile, or the columns behind N, can lie further than the size is: nothing here depends on what a difference
+  // below zero means.
   auto buffer = [&](const void* p, int64_t ld) -> __amdgpu_buffer_rsrc_t {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(static_cast<const uint16_t*>(p) + row0 * ld), 0,
                                              (int)(((rows - 1) * ld + a.N) * 2), 0x00020000);
